@@ -10,7 +10,8 @@ ABI_VERSION = 3   # include/dsp_amd.h DSP_AMD_ABI_VERSION
 
 DSP_OK, DSP_EINVAL, DSP_ESHAPE, DSP_EHIP, DSP_ENOMEM, DSP_EPARSE, DSP_EKEY, DSP_EBOUNDS = 0, -1, -2, -3, -4, -5, -6, -7
 MODULE_CODE = {"both_bilstm": 0, "seq_bilstm": 1, "signal_bilstm": 2}
-DT_F32, DT_U8, DT_U16, DT_I32 = 0, 1, 2, 3
+DT_F32, DT_U8, DT_U16, DT_I32, DT_I64 = 0, 1, 2, 3, 4
+FT_F32, FT_BF16, FT_F16 = 0, 1, 2
 INIT_ZEROS, INIT_EXPLICIT, INIT_PHILOX = 0, 1, 2
 NORM_MAD, NORM_ZSCORE = 0, 1
 PRECISION = {"fp32": 0, "fp16x3": 3, "bf16x6": 6, "bf16x9": 9}
@@ -27,6 +28,15 @@ class InitState(ctypes.Structure):
                 ("h_seq", ctypes.c_void_p), ("c_seq", ctypes.c_void_p), ("h_sig", ctypes.c_void_p),
                 ("c_sig", ctypes.c_void_p), ("h_comb", ctypes.c_void_p), ("c_comb", ctypes.c_void_p),
                 ("site_keys", ctypes.c_void_p)]
+
+
+class LstmLayer(ctypes.Structure):  # dsp_lstm_layer
+    _fields_ = ([(k, ctypes.c_int64) for k in ("batch", "steps", "input", "hidden")] + [("directions", ctypes.c_int32)] +
+                [(k, ctypes.c_void_p * 2) for k in ("w_ih", "w_hh", "b_ih", "b_hh")])
+
+
+class LstmGrads(ctypes.Structure):  # dsp_lstm_grads
+    _fields_ = [(k, ctypes.c_void_p * 2) for k in ("w_ih", "w_hh", "b_ih", "b_hh")]
 
 
 _lib = None
@@ -272,6 +282,21 @@ def lib():
     L.dsp_debug_split_bf16.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     L.dsp_debug_piece_cost.restype = ctypes.c_double
     L.dsp_debug_piece_cost.argtypes = [ctypes.POINTER(ModelCfg), ctypes.c_int32, ctypes.c_int64]
+    P, I32, I64, F, D = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
+    for name, restype, argtypes in (
+            ("dsp_embedding_forward", I32, [P, I64, P, I32, P, I64, I64, I32, F, P]),
+            ("dsp_embedding_workspace", I64, [I64, I64, I64]),
+            ("dsp_embedding_backward", I32, [P, I64, P, I32, P, I64, I64, I32, I64, F, P, P, I64]),
+            ("dsp_lstm_forward", I32, [P] * 9 + [P, I32]),
+            ("dsp_lstm_workspace", I64, [P]),
+            ("dsp_lstm_backward", I32, [P] * 15 + [P, I64]),
+            ("dsp_cross_entropy_workspace", I64, [I64]),
+            ("dsp_cross_entropy_forward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, P, P, I64]),
+            ("dsp_cross_entropy_backward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, I32, P]),
+            ("dsp_clip_workspace", I64, [I32, P]),
+            ("dsp_clip_grad_norm", I32, [P, I32, P, P, P, P, P, D, P, P, I64])):
+        fn = getattr(L, name)
+        fn.restype, fn.argtypes = restype, argtypes
     L.dsp_debug_range_probe.restype = ctypes.c_int32
     L.dsp_debug_range_probe.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]
     _lib = L

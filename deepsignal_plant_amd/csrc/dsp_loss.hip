@@ -1,0 +1,380 @@
+// dsp_loss.hip -- weighted softmax cross entropy of a batch and its gradient (the loss of train.py:75-119:
+// torch.nn.CrossEntropyLoss with a weight for each class).
+//
+//   l_n = w[y_n] (log sum_c exp x_nc - x_n,y_n)     loss = sum l_n / sum w[y_n]  (mean)  or  sum l_n  (sum)  or  l (none)
+//   dx_nc = k_n (softmax(x_n)_c - [c = y_n]),       k_n = w[y_n] / sum w[y_m]  (mean)    or  w[y_n]
+//
+// Bound by memory: every logit is read once and every gradient written once; an exponential per logit is far below what the
+// arithmetic could do meanwhile.  So a row is read into registers (it comes with its maximum and, of the values less the
+// maximum, its sum), and its gradient is written from there at once, for an upstream gradient of 1; where the backward pass
+// finds another one it computes the gradient from the logits again, so every gradient is rounded once.  Rows that do not
+// fit a workgroup's registers are read twice, the second time from the caches.
+// Rows whose label is ignore_index count for nothing and get a gradient of zeros, whatever they hold.  A label outside the
+// classes makes its row's loss and gradient NaN.  Sums over rows are held in 64 bits, in an order that the sizes decide.
+#include "dsp_ops.h"
+
+using namespace dsp;
+
+namespace {
+
+struct Loss {   // what every kernel here is given
+    const void* logits;      // [n][c], rows `stride` values apart
+    const void* labels;
+    const float* weight;     // [c] or NULL
+    void* grad;              // [n][c] or NULL
+    float* loss;             // [1], or [n] where reduction is none
+    float2* stat;            // [n]: a row's maximum m and sum of exp(x - m)
+    double* den;             // sum of the weights of all labels (mean)
+    double2* part;           // per workgroup: sum of the rows' losses, sum of their weights
+    const float* upstream;   // gradient of the loss: [1], or [n] where reduction is none
+    i64 n, c, stride, ignore;
+    int label_dtype, reduction, parts, skip_unit;
+};
+
+enum { kMean = DSP_REDUCE_MEAN, kSum = DSP_REDUCE_SUM, kNone = DSP_REDUCE_NONE };
+
+__device__ __forceinline__ i64 label_at(const Loss& p, i64 r) {
+    if (p.label_dtype == DSP_DT_I64) return ((const int64_t*)p.labels)[r];
+    if (p.label_dtype == DSP_DT_I32) return ((const int32_t*)p.labels)[r];
+    return ((const uint8_t*)p.labels)[r];
+}
+// weight of a row: 0 where it is ignored, NaN where its label is no class
+__device__ __forceinline__ float weight_of(const Loss& p, i64 y) {
+    if (y == p.ignore) return 0.0f;
+    if (y < 0 || y >= p.c) return __builtin_nanf("");
+    return p.weight ? p.weight[y] : 1.0f;
+}
+// The gradient comes from the maximum and the sum, not from their log sum exp: rounded to 32 bits that would shift every
+// probability of a row by up to |lse| 2^-24.
+// e^x as 2^(x log2 e), one hardware instruction: within 2 ulp of itself plus the rounding of the argument, |x| 2^-24
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// log sum exp of a row less its own class's logit: the difference of the logits first, where they are close it is exact
+__device__ __forceinline__ float loss_of(float m, float z, float x) { return (m - x) + logf(z); }
+
+// sum over the block's threads (a multiple of 64, at most 1,024), in every thread
+template <class T> __device__ __forceinline__ T block_sum(T x, T* scratch) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
+    __syncthreads();
+    T s = scratch[0];
+    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) s += scratch[i];
+    return s;
+}
+__device__ __forceinline__ float block_max(float x, float* scratch) {
+    x = wave_max(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float s = scratch[0];
+    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) s = fmaxf(s, scratch[i]);
+    return s;
+}
+
+// the gradient's factor of a row
+__device__ __forceinline__ float factor_of(const Loss& p, float w, i64 r) {
+    double k = w;
+    if (p.reduction == kMean) k /= *p.den;
+    if (p.upstream) k *= p.upstream[p.reduction == kNone ? r : 0];
+    return (float)k;
+}
+
+// sum of the weights of all labels: parts of the batch, then their sum
+__global__ __launch_bounds__(256) void loss_weights_kernel(Loss p) {
+    __shared__ double scratch[4];
+    double s = 0;
+    for (i64 r = (i64)blockIdx.x * 256 + threadIdx.x; r < p.n; r += (i64)gridDim.x * 256) s += weight_of(p, label_at(p, r));
+    s = block_sum(s, scratch);
+    if (threadIdx.x == 0) p.part[blockIdx.x] = make_double2(0, s);
+}
+__global__ __launch_bounds__(256) void loss_join_kernel(Loss p, int weights_only) {
+    __shared__ double scratch[4];
+    double a = 0, b = 0;
+    for (int i = threadIdx.x; i < p.parts; i += 256) {
+        a += p.part[i].x;
+        b += p.part[i].y;
+    }
+    a = block_sum(a, scratch);
+    b = block_sum(b, scratch);
+    if (threadIdx.x) return;
+    if (weights_only || p.reduction == kMean) *p.den = b;
+    if (!weights_only) *p.loss = (float)(p.reduction == kMean ? a / b : a);
+}
+
+// ---- few classes: a group of lanes (a power of two, at most 64) per row, E values a lane -----------------------------------
+template <class T, int E, bool BACKWARD>
+__global__ __launch_bounds__(256) void loss_few_kernel(Loss p, int log_lanes) {
+    __shared__ double scratch[4];
+    const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+    const i64 r = (i64)blockIdx.x * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
+    double num = 0, den = 0;
+    if (BACKWARD && p.skip_unit && p.reduction != kNone && *p.upstream == 1.0f) return;   // what the forward left is the gradient
+    if (r < p.n) {
+        const i64 y = label_at(p, r);
+        const float w = weight_of(p, y);
+        const T* row = (const T*)p.logits + r * p.stride;
+        float x[E], m = -__builtin_inff(), z = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c = lane + (e << log_lanes);
+            x[e] = c < p.c ? to_f32(row[c]) : -__builtin_inff();
+            m = fmaxf(m, x[e]);
+        }
+        if (BACKWARD) {
+            m = p.stat[r].x;
+            z = p.stat[r].y;
+        } else {
+            for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll
+            for (int e = 0; e < E; ++e) z += lane + (e << log_lanes) < p.c ? fast_exp(x[e] - m) : 0.0f;
+            for (int o = lanes >> 1; o; o >>= 1) z += __shfl_xor(z, o);
+        }
+        if (!BACKWARD && lane == 0) {
+            p.stat[r] = make_float2(m, z);
+            const float l = y != p.ignore ? w * loss_of(m, z, y >= 0 && y < p.c ? to_f32(row[y]) : 0.0f) : 0.0f;
+            if (p.reduction == kNone) p.loss[r] = l;
+            num = l;
+            den = w;
+        }
+        if (p.grad) {
+            const float k = factor_of(p, w, r);
+            const float inv = 1.0f / z;
+            T* out = (T*)p.grad + r * p.c;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int c = lane + (e << log_lanes);
+                if (c < p.c) out[c] = from_f32<T>(y == p.ignore ? 0.0f : k * (fast_exp(x[e] - m) * inv - (c == y ? 1.0f : 0.0f)));
+            }
+        }
+    }
+    if (BACKWARD || p.reduction == kNone) return;
+    num = block_sum(num, scratch);
+    den = block_sum(den, scratch);
+    if (threadIdx.x == 0) p.part[blockIdx.x] = make_double2(num, den);
+}
+
+// ---- many classes: a workgroup per row -------------------------------------------------------------------------------------
+// The row is taken as accesses of VEC values at addresses that are multiples of 16 bytes; those at its ends value by value.
+// R > 0: up to R accesses a thread, held in registers; R = 0: any number, read twice.
+template <class T, int VEC> struct RowOf {
+    typedef Vec<T, VEC> V;
+    const T* row;
+    T* out;
+    int shift;   // values between the aligned address before the row and the row
+    int c;
+    __device__ __forceinline__ int accesses() const { return (c + shift + VEC - 1) / VEC; }
+    __device__ __forceinline__ V load(int j) const {
+        const int at = j * VEC - shift;
+        if (VEC > 1 && at >= 0 && at + VEC <= c) return *(const V*)(row + at);
+        V x;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x.v[e] = at + e >= 0 && at + e < c ? row[at + e] : (T)(-__builtin_inff());
+        return x;
+    }
+    __device__ __forceinline__ void store(int j, const V& x) const {
+        const int at = j * VEC - shift;
+        if (VEC > 1 && at >= 0 && at + VEC <= c) {
+            *(V*)(out + at) = x;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (at + e >= 0 && at + e < c) out[at + e] = x.v[e];
+    }
+    __device__ __forceinline__ bool inside(int j, int e) const { return j * VEC - shift + e >= 0 && j * VEC - shift + e < c; }
+};
+
+template <class T, int VEC, int R, bool BACKWARD>
+__global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
+    typedef Vec<T, VEC> V;
+    __shared__ float scratch[16];
+    if (BACKWARD && p.skip_unit && p.reduction != kNone && *p.upstream == 1.0f) return;
+    const i64 r = blockIdx.x;
+    const i64 y = label_at(p, r);
+    const float w = weight_of(p, y);
+    const int threads = blockDim.x;
+    RowOf<T, VEC> row;
+    row.row = (const T*)p.logits + r * p.stride;
+    row.out = (T*)p.grad + r * p.c;
+    row.shift = VEC > 1 ? (int)((size_t)row.row % 16 / sizeof(T)) : 0;
+    row.c = (int)p.c;
+    const int n = row.accesses();
+    if (y == p.ignore) {   // nothing to read
+        if (!BACKWARD && threadIdx.x == 0) {
+            p.stat[r] = make_float2(0.0f, 1.0f);
+            if (p.reduction == kNone) p.loss[r] = 0.0f;
+            else p.part[r] = make_double2(0, 0);
+        }
+        V none;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) none.v[e] = T{};
+        if (p.grad)
+            for (int j = threadIdx.x; j < n; j += threads) row.store(j, none);
+        return;
+    }
+    V x[R ? R : 1];
+    float m = -__builtin_inff(), z = 0.0f;
+    if (R) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int j = threadIdx.x + i * threads;
+            if (j < n) x[i] = row.load(j);
+        }
+    }
+    if (BACKWARD) {
+        m = p.stat[r].x;
+        z = p.stat[r].y;
+    } else {
+        if (R) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if ((int)threadIdx.x + i * threads < n)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) m = fmaxf(m, to_f32(x[i].v[e]));
+            m = block_max(m, scratch);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int j = threadIdx.x + i * threads;
+                if (j < n)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) z += row.inside(j, e) ? fast_exp(to_f32(x[i].v[e]) - m) : 0.0f;
+            }
+        } else {
+            // one pass with a running maximum: what was summed under the old one is scaled when it moves
+            for (int j = threadIdx.x; j < n; j += threads) {
+                const V v = row.load(j);
+                float top = m;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) top = fmaxf(top, to_f32(v.v[e]));
+                if (top > m) {
+                    z *= fast_exp(m - top);   // m = -inf at first: 0
+                    m = top;
+                }
+                if (m > -__builtin_inff())
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) z += row.inside(j, e) ? fast_exp(to_f32(v.v[e]) - m) : 0.0f;
+                else
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) z += to_f32(v.v[e]) == m ? 0.0f : __builtin_nanf("");   // nothing but -inf so far, or a NaN
+            }
+            const float top = block_max(m, scratch);
+            z = m == top ? z : z * fast_exp(m - top);
+            m = top;
+        }
+        z = block_sum(z, scratch);
+        if (m == -__builtin_inff()) z = __builtin_nanf("");   // no class is possible
+        if (threadIdx.x == 0) {
+            p.stat[r] = make_float2(m, z);
+            const float l = w * loss_of(m, z, y >= 0 && y < p.c ? to_f32(row.row[y]) : 0.0f);
+            if (p.reduction == kNone) p.loss[r] = l;
+            else p.part[r] = make_double2(l, w);
+        }
+    }
+    if (!p.grad) return;
+    const float k = factor_of(p, w, r), inv = 1.0f / z;
+    auto gradient = [&](int j, V v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            v.v[e] = from_f32<T>(k * (fast_exp(to_f32(v.v[e]) - m) * inv - (j * VEC - row.shift + e == y ? 1.0f : 0.0f)));
+        row.store(j, v);
+    };
+    if (R) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int j = threadIdx.x + i * threads;
+            if (j < n) gradient(j, x[i]);
+        }
+    } else
+        for (int j = threadIdx.x; j < n; j += threads) gradient(j, row.load(j));
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------
+constexpr i64 kFew = 256;   // classes up to which a row is a group of lanes' work
+
+template <class T, bool BACKWARD> i64 launch_rows(hipStream_t s, const Loss& p) {
+    if (p.c <= kFew) {
+        int ll = 0;
+        while ((4 << ll) < p.c) ++ll;   // 4 values a lane
+        const i64 blocks = cdiv(p.n, 256 >> ll);
+        hipLaunchKernelGGL((loss_few_kernel<T, 4, BACKWARD>), dim3((unsigned)blocks), dim3(256), 0, s, p, ll);
+        return blocks;
+    }
+    constexpr int W = 16 / sizeof(T);
+    // wide accesses for the gradient too: its rows must begin at the same place within 16 bytes as the logits' rows
+    const bool wide = !p.grad || ((size_t)p.logits % 16 == (size_t)p.grad % 16 && (p.n == 1 || (p.stride - p.c) * (i64)sizeof(T) % 16 == 0));
+    const i64 vecs = wide ? cdiv(p.c, W) + 1 : p.c;
+    const int threads = vecs <= 256 ? 256 : vecs <= 1024 ? 512 : 1024;
+    const int per = (int)cdiv(vecs, threads);
+#define DSP_ROW(VEC, R) hipLaunchKernelGGL((loss_many_kernel<T, VEC, R, BACKWARD>), dim3((unsigned)p.n), dim3(threads), 0, s, p)
+    if (wide) {
+        if (per <= 1) DSP_ROW(W, 1);
+        else if (per <= 2) DSP_ROW(W, 2);
+        else if (per <= 4) DSP_ROW(W, 4);
+        else if (per <= 8) DSP_ROW(W, 8);
+        else DSP_ROW(W, 0);
+    } else {
+        if (per <= 8) DSP_ROW(1, 8);
+        else DSP_ROW(1, 0);
+    }
+#undef DSP_ROW
+    return p.n;
+}
+template <bool BACKWARD> i64 launch_typed(hipStream_t s, const Loss& p, int dtype) {
+    if (dtype == DSP_FT_F32) return launch_rows<float, BACKWARD>(s, p);
+    if (dtype == DSP_FT_BF16) return launch_rows<__bf16, BACKWARD>(s, p);
+    return launch_rows<_Float16, BACKWARD>(s, p);
+}
+
+const char* bad_loss(i64 n, i64 c, i64 stride, int dtype, int label_dtype, int reduction) {
+    if (n < 0 || n > 0x7fffffffll) return "the number of rows must be within 0 .. 2^31 - 1";
+    if (c < 1 || c > (1ll << 30)) return "the number of classes must be within 1 .. 2^30";
+    if (stride < c && n > 1) return "rows overlap: the row stride is below the number of classes";
+    if (dtype != DSP_FT_F32 && dtype != DSP_FT_BF16 && dtype != DSP_FT_F16) return "unknown element type";
+    if (label_dtype != DSP_DT_I64 && label_dtype != DSP_DT_I32 && label_dtype != DSP_DT_U8) return "labels must be int64, int32 or uint8";
+    if (reduction != kMean && reduction != kSum && reduction != kNone) return "unknown reduction";
+    return nullptr;
+}
+constexpr i64 kWeightParts = 256;
+i64 parts_of(i64 n) { return n > kWeightParts ? n : kWeightParts; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)(parts_of(n) * sizeof(double2)); }
+
+int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride, const void* labels,
+                                  int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction, float* loss, float* stat,
+                                  double* weight_sum, void* grad, void* workspace, int64_t workspace_bytes) {
+    const char* who = "dsp_cross_entropy_forward";
+    if (const char* why = bad_loss(n, c, row_stride, dtype, label_dtype, reduction)) return refuse(who, why);
+    if (!workspace || workspace_bytes < dsp_cross_entropy_workspace(n)) return refuse(who, "workspace too small (dsp_cross_entropy_workspace)");
+    if (n && (!logits || !labels || !loss || !stat)) return refuse(who, "NULL pointer");
+    if ((reduction != kNone && !loss) || (reduction == kMean && !weight_sum)) return refuse(who, "NULL pointer");
+    Loss p = {logits, labels, weight, grad, loss, (float2*)stat, weight_sum, (double2*)workspace, nullptr, n, c, row_stride, ignore_index, label_dtype, reduction, 0, 0};
+    hipStream_t s = (hipStream_t)stream;
+    if (grad && reduction == kMean && n) {   // the gradient's factor is known before its rows are
+        p.parts = (int)(cdiv(n, 256) < kWeightParts ? cdiv(n, 256) : kWeightParts);
+        hipLaunchKernelGGL(loss_weights_kernel, dim3(p.parts), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(256), 0, s, p, 1);
+    }
+    p.parts = n ? (int)launch_typed<false>(s, p, dtype) : 0;
+    if (reduction != kNone) hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(256), 0, s, p, 0);
+    return launched(who);
+}
+
+int32_t dsp_cross_entropy_backward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride, const void* labels,
+                                   int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction, const float* stat,
+                                   const double* weight_sum, const float* upstream, int32_t skip_unit, void* grad) {
+    const char* who = "dsp_cross_entropy_backward";
+    if (const char* why = bad_loss(n, c, row_stride, dtype, label_dtype, reduction)) return refuse(who, why);
+    if (n == 0) return DSP_OK;
+    if (!logits || !labels || !stat || !upstream || !grad || (reduction == kMean && !weight_sum)) return refuse(who, "NULL pointer");
+    Loss p = {logits, labels, weight, grad, nullptr, (float2*)stat, (double*)weight_sum, nullptr, upstream, n, c, row_stride, ignore_index, label_dtype,
+              reduction, 0, skip_unit};
+    launch_typed<true>((hipStream_t)stream, p, dtype);
+    return launched(who);
+}
+
+}  // extern "C"

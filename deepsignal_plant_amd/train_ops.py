@@ -1,0 +1,389 @@
+"""The operators of a training step over the gfx950 kernels: what the reference's `train` (train.py:75-119) takes from torch
+around ModelBiLSTM.
+
+  embedding        lookup with scaling, gradient by sorted tokens             (nn.Embedding, models.py:186)
+  lstm             one layer, one or both directions                          (nn.LSTM, models.py:137-157)
+  cross_entropy    softmax cross entropy with class weights                   (nn.CrossEntropyLoss)
+  clip_grad_norm_  clipping by the norm over many gradients, in place         (nn.utils.clip_grad_norm_)
+  clip_grad_norm   the same into other tensors;  grad_norm: the norm alone
+
+The first three are differentiable once by torch's autograd.  Everything runs on the tensors' GPU and its current stream,
+enqueues kernels only (no copy, no synchronisation; workspaces come from torch's allocator, so a captured call's belong to its
+graph) and gives the same bits for the same inputs and sizes.  There is no CPU path.  ValueError for shapes, types and values;
+RuntimeError for tensors that are not on one GPU."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+
+_FLOAT = {torch.float32: nat.FT_F32, torch.bfloat16: nat.FT_BF16, torch.float16: nat.FT_F16}
+_TOKEN = {torch.float32: nat.DT_F32, torch.uint8: nat.DT_U8, torch.uint16: nat.DT_U16, torch.int32: nat.DT_I32, torch.int64: nat.DT_I64}
+_LABEL = {torch.uint8: nat.DT_U8, torch.int32: nat.DT_I32, torch.int64: nat.DT_I64}
+_REDUCE = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _one_gpu(who, *tensors):
+    """the tensors' GPU (None among them: not given)"""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s: expected a tensor, got %s" % (who, type(t).__name__))
+        if not t.is_cuda:
+            raise RuntimeError("%s: tensors must live on a GPU (no CPU path)" % who)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError("%s: tensors on %s and %s" % (who, dev, t.device))
+    return dev
+
+
+def _call(dev, fn, *args):
+    """one call of the library on `dev` and its current stream"""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        return nat.check(fn(stream, *args))
+    with torch.cuda.device(dev):
+        return nat.check(fn(stream, *args))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(dev, size):
+    return torch.empty(nat.check(size), dtype=torch.uint8, device=dev)
+
+
+# ---- embedding ----------------------------------------------------------------------------------------------------------------
+def _embedding_forward(tokens, weight, scale):
+    out = torch.empty(tokens.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
+    _call(weight.device, nat.lib().dsp_embedding_forward, tokens.numel(), tokens.data_ptr(), _TOKEN[tokens.dtype], weight.data_ptr(), weight.shape[0],
+          weight.shape[1], _FLOAT[weight.dtype], scale, out.data_ptr())
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding_idx):
+        ctx.save_for_backward(tokens)
+        ctx.table, ctx.scale, ctx.padding_idx = weight.shape, scale, padding_idx
+        return _embedding_forward(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        tokens, = ctx.saved_tensors
+        (vocab, dim), n, L = ctx.table, tokens.numel(), nat.lib()
+        grad = grad.contiguous()
+        out = torch.empty(ctx.table, dtype=grad.dtype, device=grad.device)
+        ws = _workspace(grad.device, L.dsp_embedding_workspace(n, vocab, dim))
+        _call(grad.device, L.dsp_embedding_backward, n, tokens.data_ptr(), _TOKEN[tokens.dtype], grad.data_ptr(), vocab, dim, _FLOAT[grad.dtype],
+              ctx.padding_idx, ctx.scale, out.data_ptr(), ws.data_ptr(), ws.numel())
+        return None, out, None, None
+
+
+def embedding(tokens, weight, scale=1.0, padding_idx=None):
+    """scale * weight[tokens]: [..., dim] for tokens of any shape and weight [rows, dim] (float32, bfloat16 or float16).
+
+    tokens: uint8, uint16, int32, int64, or float32 as the reference feeds k-mer codes (cut towards zero).  A token outside the
+    table gives a row of NaN and no gradient.  padding_idx: that row of the table gets no gradient (negative: from the end).
+    Products and the gradient's sums are held in 32 bits and rounded once."""
+    _one_gpu("embedding", tokens, weight)
+    if tokens.dtype not in _TOKEN:
+        raise ValueError("embedding: tokens must be uint8, uint16, int32, int64 or float32, got %s" % tokens.dtype)
+    if weight.dtype not in _FLOAT or weight.dim() != 2:
+        raise ValueError("embedding: weight must be [rows, dim] in float32, bfloat16 or float16, got %s %s" % (list(weight.shape), weight.dtype))
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("embedding: scale must be finite")
+    pad = -1
+    if padding_idx is not None:
+        pad = int(padding_idx)
+        if not -weight.shape[0] <= pad < weight.shape[0]:
+            raise ValueError("embedding: padding_idx %d is not a row of the table" % pad)
+        pad %= weight.shape[0]
+    tokens = tokens.detach().contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(tokens, weight.contiguous(), scale, pad)
+    return _embedding_forward(tokens, weight.detach().contiguous(), scale)
+
+
+# ---- lstm -----------------------------------------------------------------------------------------------------------------------
+def _layer(x, weights):
+    hidden = weights[1].shape[1]
+    l = nat.LstmLayer(x.shape[0], x.shape[1], x.shape[2], hidden, len(weights) // 4)
+    for d in range(l.directions):
+        l.w_ih[d], l.w_hh[d], l.b_ih[d], l.b_hh[d] = (w.data_ptr() for w in weights[4 * d:4 * d + 4])
+    return l
+
+
+def _lstm_forward(x, h0, c0, weights, save):
+    l, dev = _layer(x, weights), x.device
+    B, T, H, D = l.batch, l.steps, l.hidden, l.directions
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
+    y, hn, cn, gates, cells = new(B, T, D * H), new(D, B, H), new(D, B, H), new(D, T, B, 4 * H), new(D, T if save else 2, B, H)
+    _call(dev, nat.lib().dsp_lstm_forward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), hn.data_ptr(), cn.data_ptr(), gates.data_ptr(),
+          cells.data_ptr(), int(save))
+    return y, hn, cn, gates, cells
+
+
+class _Lstm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h0, c0, *weights):
+        y, hn, cn, gates, cells = _lstm_forward(x, h0, c0, weights, True)
+        ctx.save_for_backward(x, h0, c0, y, gates, cells, *weights)
+        ctx.set_materialize_grads(False)
+        return y, hn, cn
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, ghn, gcn):
+        x, h0, c0, y, gates, cells, *weights = ctx.saved_tensors
+        l, dev, L = _layer(x, weights), x.device, nat.lib()
+        gy, ghn, gcn = (None if g is None else g.contiguous() for g in (gy, ghn, gcn))
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        states = (l.directions, l.batch, l.hidden)
+        dh0 = torch.empty(states, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
+        dc0 = torch.empty(states, dtype=torch.float32, device=dev)
+        dws = [torch.empty_like(w) for w in weights]
+        g = nat.LstmGrads()
+        for d in range(l.directions):
+            g.w_ih[d], g.w_hh[d], g.b_ih[d], g.b_hh[d] = (w.data_ptr() for w in dws[4 * d:4 * d + 4])
+        ws = _workspace(dev, L.dsp_lstm_workspace(ctypes.byref(l)))
+        _call(dev, L.dsp_lstm_backward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), gates.data_ptr(), cells.data_ptr(), _ptr(gy),
+              _ptr(ghn), _ptr(gcn), _ptr(dx), _ptr(dh0), dc0.data_ptr(), ctypes.byref(g), ws.data_ptr(), ws.numel())
+        return (dx, dh0, dc0 if ctx.needs_input_grad[2] else None, *dws)
+
+
+def lstm(x, weights, h0=None, c0=None):
+    """One LSTM layer: (y [batch, steps, directions * hidden], hn, cn [directions, batch, hidden]) of x [batch, steps, input], as
+    torch.nn.LSTM(batch_first=True).  float32 only.
+
+    weights: weight_ih [4 * hidden, input], weight_hh [4 * hidden, hidden], bias_ih, bias_hh [4 * hidden], and the same four of the
+    reverse direction for a bidirectional layer (the order of the state_dict; gates i, f, g, o).  h0, c0 [directions, batch,
+    hidden]: zeros where not given.  One step with the states handed on is the form for running sequences.  The gradient costs
+    memory of 9 * hidden values a step, sequence and direction from the forward to the backward pass; under torch.no_grad none."""
+    weights = list(weights)
+    if len(weights) not in (4, 8):
+        raise ValueError("lstm: expected the 4 weights of one direction or the 8 of two, got %d" % len(weights))
+    _one_gpu("lstm", x, h0, c0, *weights)
+    for t in (x, h0, c0, *weights):
+        if t is not None and t.dtype != torch.float32:
+            raise ValueError("lstm: tensors must be float32, got %s" % t.dtype)
+    if x.dim() != 3 or weights[1].dim() != 2:
+        raise ValueError("lstm: x must be [batch, steps, input] and weight_hh [4 * hidden, hidden]")
+    hidden, dirs = weights[1].shape[1], len(weights) // 4
+    want = [(4 * hidden, x.shape[2]), (4 * hidden, hidden), (4 * hidden,), (4 * hidden,)] * dirs
+    for w, shape in zip(weights, want):
+        if tuple(w.shape) != shape:
+            raise ValueError("lstm: a weight has shape %s, expected %s" % (tuple(w.shape), shape))
+    for name, t in (("h0", h0), ("c0", c0)):
+        if t is not None and tuple(t.shape) != (dirs, x.shape[0], hidden):
+            raise ValueError("lstm: %s has shape %s, expected %s" % (name, tuple(t.shape), (dirs, x.shape[0], hidden)))
+    x, h0, c0 = (None if t is None else t.contiguous() for t in (x, h0, c0))
+    weights = [w.contiguous() for w in weights]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h0, c0, *weights)):
+        return _Lstm.apply(x, h0, c0, *weights)
+    return _lstm_forward(x, h0, c0, weights, False)[:3]
+
+
+# ---- cross entropy ---------------------------------------------------------------------------------------------------------------
+def _loss_args(logits, labels, weight, ignore_index, reduction):
+    return (logits.shape[0], logits.shape[1], logits.data_ptr(), _FLOAT[logits.dtype], logits.stride(0), labels.data_ptr(), _LABEL[labels.dtype], _ptr(weight),
+            ignore_index, reduction)
+
+
+def _loss_forward(logits, labels, weight, ignore_index, reduction, want_grad):
+    dev, n, L = logits.device, logits.shape[0], nat.lib()
+    loss = torch.empty((n,) if reduction == 2 else (), dtype=torch.float32, device=dev)
+    stat = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    total = torch.empty((), dtype=torch.float64, device=dev)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad and reduction != 2 else None
+    ws = _workspace(dev, L.dsp_cross_entropy_workspace(n))
+    _call(dev, L.dsp_cross_entropy_forward, *_loss_args(logits, labels, weight, ignore_index, reduction), loss.data_ptr(), stat.data_ptr(), total.data_ptr(),
+          _ptr(grad), ws.data_ptr(), ws.numel())
+    return loss, stat, total, grad
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, weight, ignore_index, reduction):
+        loss, stat, total, ctx.unit_grad = _loss_forward(logits, labels, weight, ignore_index, reduction, True)
+        ctx.save_for_backward(logits, labels, weight, stat, total)
+        ctx.how = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        logits, labels, weight, stat, total = ctx.saved_tensors
+        # the gradient that the forward pass left is handed out once; a second pass over a retained graph computes its own
+        grad, ctx.unit_grad = ctx.unit_grad, None
+        unit = grad is not None
+        if not unit:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        upstream = upstream.contiguous()
+        _call(logits.device, nat.lib().dsp_cross_entropy_backward, *_loss_args(logits, labels, weight, *ctx.how), stat.data_ptr(), total.data_ptr(),
+              upstream.data_ptr(), int(unit), grad.data_ptr())
+        return grad, None, None, None, None
+
+
+def cross_entropy(logits, labels, weight=None, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of logits [n, classes] (float32, bfloat16, float16) against labels [n] (int64, int32, uint8), as
+    torch.nn.functional.cross_entropy with class indices; the loss is float32.
+
+    weight [classes] float32: weight of each class.  Rows labelled ignore_index count for nothing, whatever they hold, and get a
+    gradient of zeros; reduction "mean" divides by the sum of the other labels' weights (NaN where there are none).  A label that
+    is no class makes its row's loss and gradient NaN.  Where the logits require a gradient it is computed with the loss, for
+    an upstream gradient of 1; another one makes the backward pass compute it again from the logits."""
+    _one_gpu("cross_entropy", logits, labels, weight)
+    if logits.dim() != 2 or logits.dtype not in _FLOAT or logits.shape[1] < 1:
+        raise ValueError("cross_entropy: logits must be [n, classes] in float32, bfloat16 or float16, got %s %s" % (list(logits.shape), logits.dtype))
+    if tuple(labels.shape) != (logits.shape[0],) or labels.dtype not in _LABEL:
+        raise ValueError("cross_entropy: labels must be [%d] in int64, int32 or uint8, got %s %s" % (logits.shape[0], list(labels.shape), labels.dtype))
+    if weight is not None and (tuple(weight.shape) != (logits.shape[1],) or weight.dtype != torch.float32):
+        raise ValueError("cross_entropy: weight must be [%d] in float32, got %s %s" % (logits.shape[1], list(weight.shape), weight.dtype))
+    if weight is not None and weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError("cross_entropy: no gradient is computed for the class weights")
+    if reduction not in _REDUCE:
+        raise ValueError("cross_entropy: reduction must be 'mean', 'sum' or 'none'")
+    n, c = logits.shape
+    if (c > 1 and logits.stride(1) != 1) or (n > 1 and logits.stride(0) < c):
+        logits = logits.contiguous()
+    labels, weight, how = labels.contiguous(), None if weight is None else weight.detach().contiguous(), _REDUCE[reduction]
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _CrossEntropy.apply(logits, labels, weight, int(ignore_index), how)
+    return _loss_forward(logits, labels, weight, int(ignore_index), how, False)[0]
+
+
+# ---- the norm of many gradients -----------------------------------------------------------------------------------------------
+def _is_dense(t):
+    """whether the values fill one piece of memory, in whatever order"""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+def _check_grads(who, grads):
+    for g in grads:
+        if not isinstance(g, torch.Tensor) or g.layout != torch.strided:
+            raise ValueError("%s: gradients must be dense tensors" % who)
+        if g.dtype not in _FLOAT:
+            raise ValueError("%s: gradients must be float32, bfloat16 or float16, got %s" % (who, g.dtype))
+    return _one_gpu(who, *grads)
+
+
+def _spans(tensors):
+    return [(p, p + t.numel() * t.element_size()) for t in tensors for p in (t.data_ptr(),) if t.numel()]
+
+
+def _check_apart(who, spans):
+    spans.sort()
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise ValueError("%s: tensors that are written overlap in memory" % who)
+
+
+def _run_clip(dev, grads, outs, max_norm):
+    n = len(grads)
+    ptr, i64, i32 = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int32 * n
+    numels = i64(*[g.numel() for g in grads])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    L = nat.lib()
+    ws = _workspace(dev, L.dsp_clip_workspace(n, numels))
+    _call(dev, L.dsp_clip_grad_norm, n, ptr(*[g.data_ptr() for g in grads]), numels, i32(*[_FLOAT[g.dtype] for g in grads]),
+          None if outs is None else ptr(*[o.data_ptr() for o in outs]), None if outs is None else i32(*[_FLOAT[o.dtype] for o in outs]), max_norm,
+          norm.data_ptr(), ws.data_ptr(), ws.numel())
+    return norm
+
+
+def _max_norm(who, max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("%s: max_norm must not be negative" % who)
+    return max_norm
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """The 2-norm over all values of a list of tensors, as a float32 scalar on their GPU; squares and sums are held in 64 bits."""
+    grads = list(grads)
+    dev = _check_grads("grad_norm", grads)
+    if dev is None:
+        raise ValueError("grad_norm: no tensors")
+    return _run_clip(dev, [g if _is_dense(g) else g.contiguous() for g in grads], None, 0.0)
+
+
+@torch.no_grad()
+def clip_grad_norm(grads, max_norm, out=None):
+    """(norm, clipped): min(1, max_norm / (norm + 1e-6)) times every gradient, written into other tensors.
+
+    out: one contiguous tensor for each gradient, of its shape, in its type or in float32 (the gradients an optimizer with
+    32-bit weights takes); new ones where it is not given.  The gradients are left as they are."""
+    who, grads = "clip_grad_norm", list(grads)
+    max_norm = _max_norm(who, max_norm)
+    dev = _check_grads(who, grads)
+    if dev is None:
+        raise ValueError("clip_grad_norm: no tensors")
+    out = [torch.empty(g.shape, dtype=g.dtype, device=dev) for g in grads] if out is None else list(out)
+    if len(out) != len(grads):
+        raise ValueError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
+    _one_gpu(who, grads[0], *out)
+    for g, o in zip(grads, out):
+        if o.shape != g.shape or not o.is_contiguous() or (o.dtype != g.dtype and o.dtype != torch.float32):
+            raise ValueError("clip_grad_norm: an output must be contiguous, of its gradient's shape, and of its type or float32")
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    outs = _spans(out)
+    _check_apart(who, outs)
+    ins, i = sorted(_spans(grads)), 0
+    for start, end in outs:   # both in order of their addresses, the outputs apart from each other
+        while i < len(ins) and ins[i][1] <= start:
+            i += 1
+        if i < len(ins) and ins[i][0] < end:
+            raise ValueError("clip_grad_norm: an output overlaps a gradient (clip_grad_norm_ works in place)")
+    return _run_clip(dev, grads, out, max_norm), out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scale the gradients of `parameters` (a tensor or an iterable of them) in place so that their 2-norm over all values is at
+    most max_norm, as torch.nn.utils.clip_grad_norm_; returns the norm before, a float32 scalar on their GPU.
+
+    The gradients may be of different types and sizes, all on one GPU.  A gradient that two parameters share counts once.  Where
+    there is nothing to clip they are read but not written.  error_if_nonfinite waits for the norm and raises RuntimeError
+    before anything is changed."""
+    who = "clip_grad_norm_"
+    if float(norm_type) != 2.0:
+        raise ValueError("clip_grad_norm_: norm_type must be 2")
+    max_norm = _max_norm(who, max_norm)
+    grads = [p.grad for p in ((parameters,) if isinstance(parameters, torch.Tensor) else parameters) if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    dev = _check_grads(who, grads)
+    grads = list({(g.data_ptr(), g.shape, g.stride(), g.dtype): g for g in grads}.values())
+    use = [g if _is_dense(g) else g.contiguous() for g in grads]
+    for g, u in zip(grads, use):
+        if u is not g and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
+    _check_apart(who, _spans(use))
+    if error_if_nonfinite:
+        norm = _run_clip(dev, use, None, 0.0)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError("clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped")
+    norm = _run_clip(dev, use, use, max_norm)
+    for g, u in zip(grads, use):
+        if u is not g:
+            g.copy_(u)
+    return norm

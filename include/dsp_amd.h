@@ -550,6 +550,88 @@ double dsp_debug_piece_cost(const dsp_model_cfg* cfg, int32_t n_cus, int64_t n_s
  * address there), out[3] = floats of the 4 KiB buffer still 1.0 after 64 out-of-range stores (1,024: dropped). */
 int32_t dsp_debug_range_probe(int32_t device, int32_t out[4]);
 
+/* ---- the operators of a training step (csrc/dsp_embed.hip, dsp_lstm_train.hip, dsp_loss.hip, dsp_clip.hip) ------------------
+ * What the reference's `train` (train.py:75-119) computes with torch's own operators around ModelBiLSTM: the embedding
+ * lookup (models.py:186), the LSTM layers (models.py:137-157), CrossEntropyLoss with class weights, and
+ * clip_grad_norm_, each with its gradient.  deepsignal_plant_amd/train_ops.py is the Python side.
+ *
+ * All pointers but the argument structs, the tables of dsp_clip_grad_norm and the weight tables in dsp_lstm_layer are DEVICE
+ * pointers on the device that is current, to contiguous arrays unless a stride is given; outputs overlap nothing else (but
+ * in place where it says so).  Calls only enqueue kernels on `stream`: no copy, no allocation, no synchronisation, no state,
+ * so any number may run at once, each with its own workspace (aligned to 256 bytes, free again when the call's kernels are
+ * done), and all may be captured.  Results do not depend on timing: no floating-point atomics.  Where a workspace is asked
+ * for, the matching function gives its size in bytes for the same sizes (negative: a dsp_status).  DSP_EINVAL with a message
+ * for anything refused; nothing is enqueued then. */
+
+/* element types of these operators; token / label types are DSP_DT_* with */
+enum { DSP_FT_F32 = 0, DSP_FT_BF16 = 1, DSP_FT_F16 = 2 };
+enum { DSP_DT_I64 = 4 };
+
+/* out[n][dim] = scale * weight[tokens[n]][dim].  A token outside the table gives a row of NaN (visible, never another token's
+ * row).  float32 tokens (the reference's convention) are cut towards zero.  n <= 2^31 - 1, dim <= 65,536; products in 32 bits. */
+int32_t dsp_embedding_forward(void* stream, int64_t n, const void* tokens, int32_t token_dtype, const void* weight, int64_t vocab,
+                              int64_t dim, int32_t dtype, float scale, void* out);
+/* weight_grad[vocab][dim] = scale * sums of grad[n][dim] by token: all rows are written.  Tokens outside the table and, unless it
+ * is -1, tokens equal to padding_idx count for nothing.  Sums in 32 bits. */
+int64_t dsp_embedding_workspace(int64_t n, int64_t vocab, int64_t dim);
+int32_t dsp_embedding_backward(void* stream, int64_t n, const void* tokens, int32_t token_dtype, const void* grad, int64_t vocab,
+                               int64_t dim, int32_t dtype, int64_t padding_idx, float scale, void* weight_grad, void* workspace,
+                               int64_t workspace_bytes);
+
+/* One LSTM layer of one or two directions, fp32: torch.nn.LSTM(batch_first=True) with its gates i, f, g, o along 4 * hidden.
+ * w_ih [4 hidden][input], w_hh [4 hidden][hidden], b_ih, b_hh [4 hidden] of each direction ([1]: the reverse one). */
+typedef struct dsp_lstm_layer {
+    int64_t batch, steps, input, hidden;
+    int32_t directions;
+    const float* w_ih[2];
+    const float* w_hh[2];
+    const float* b_ih[2];
+    const float* b_hh[2];
+} dsp_lstm_layer;
+typedef struct dsp_lstm_grads {   /* of the same shapes; b_ih and b_hh get the same values */
+    float* w_ih[2];
+    float* w_hh[2];
+    float* b_ih[2];
+    float* b_hh[2];
+} dsp_lstm_grads;
+/* x [batch][steps][input]; h0, c0 [directions][batch][hidden] or NULL (zeros) -> y [batch][steps][directions * hidden], hn, cn
+ * [directions][batch][hidden].  gates: [directions][steps][batch][4 hidden] scratch.  save = 1 keeps what the backward pass needs in
+ * gates and in cells [directions][steps][batch][hidden]; save = 0: cells is scratch of [directions][2][batch][hidden].
+ * batch 0 is allowed; steps 1 is the single step of a running sequence. */
+int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* layer, const float* x, const float* h0, const float* c0, float* y, float* hn,
+                         float* cn, float* gates, float* cells, int32_t save);
+/* gradients of x (dx NULL: not wanted), h0 (dh0 NULL: not wanted), c0 (always written) and all weights, from those of y, hn and
+ * cn (each may be NULL: zeros).  gates and cells as a forward pass with save = 1 left them; they are only read. */
+int64_t dsp_lstm_workspace(const dsp_lstm_layer* layer);
+int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* layer, const float* x, const float* h0, const float* c0, const float* y,
+                          const float* gates, const float* cells, const float* grad_y, const float* grad_hn, const float* grad_cn,
+                          float* dx, float* dh0, float* dc0, const dsp_lstm_grads* grads, void* workspace, int64_t workspace_bytes);
+
+/* Softmax cross entropy of n rows of c logits (rows row_stride values apart) with an optional weight per class, as
+ * torch.nn.CrossEntropyLoss: reduction MEAN divides by the sum of the labels' weights (NaN where there are none), NONE
+ * gives a loss per row.  Rows labelled ignore_index count for nothing, whatever they hold; a label outside the classes makes its row NaN.
+ * loss: [1], or [n] (NONE).  stat [n][2] (a row's maximum, its sum of exp(x - maximum)) and weight_sum [1] are kept for the
+ * backward pass.  grad, if not NULL, [n][c] contiguous: the gradient of the logits for an upstream gradient of 1 (not with NONE). */
+enum { DSP_REDUCE_MEAN = 0, DSP_REDUCE_SUM = 1, DSP_REDUCE_NONE = 2 };
+int64_t dsp_cross_entropy_workspace(int64_t n);
+int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride,
+                                  const void* labels, int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction,
+                                  float* loss, float* stat, double* weight_sum, void* grad, void* workspace, int64_t workspace_bytes);
+/* grad [n][c] = the gradient for upstream [1] ([n] with NONE).  skip_unit: grad holds the forward pass's gradient already, and
+ * where upstream is 1 (read on the device) it is left as it is. */
+int32_t dsp_cross_entropy_backward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride,
+                                   const void* labels, int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction,
+                                   const float* stat, const double* weight_sum, const float* upstream, int32_t skip_unit, void* grad);
+
+/* norm [1] = the 2-norm over all values of n_tensors arrays; outs (NULL: the norm alone) = min(1, max_norm / (norm + 1e-6)) times
+ * them.  grads, outs, numels, dtypes, out_dtypes are HOST tables; an output has its gradient's type or float32, and may be its
+ * gradient itself (it is then left alone where there is nothing to clip).  Arrays may begin anywhere their element type allows.
+ * A norm that is NaN makes every output NaN, an infinite one makes them 0 (NaN where they were infinite). */
+int64_t dsp_clip_workspace(int32_t n_tensors, const int64_t* numels);
+int32_t dsp_clip_grad_norm(void* stream, int32_t n_tensors, const void* const* grads, const int64_t* numels, const int32_t* dtypes,
+                           void* const* outs, const int32_t* out_dtypes, double max_norm, float* norm, void* workspace,
+                           int64_t workspace_bytes);
+
 const char* dsp_last_error(void);
 int32_t dsp_abi_version(void);
 
