@@ -289,7 +289,7 @@ def lib():
             ("dsp_embedding_backward", I32, [P, I64, P, I32, P, I64, I64, I32, I64, F, P, P, I64]),
             ("dsp_lstm_forward", I32, [P] * 9 + [P, I32]),
             ("dsp_lstm_workspace", I64, [P]),
-            ("dsp_lstm_backward", I32, [P] * 15 + [P, I64]),
+            ("dsp_lstm_backward", I32, [P] * 13 + [P, I64]),
             ("dsp_cross_entropy_workspace", I64, [I64]),
             ("dsp_cross_entropy_forward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, P, P, I64]),
             ("dsp_cross_entropy_backward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, I32, P]),

@@ -29,6 +29,8 @@ struct Loss {   // what every kernel here is given
     const float* upstream;   // gradient of the loss: [1], or [n] where reduction is none
     i64 n, c, stride, ignore;
     int label_dtype, reduction, parts, skip_unit;
+    double* weight_part;     // [weight_parts]: sums of labels' weights;  weight_parts 0: den holds their sum, if it is wanted
+    int weight_parts;
 };
 
 enum { kMean = DSP_REDUCE_MEAN, kSum = DSP_REDUCE_SUM, kNone = DSP_REDUCE_NONE };
@@ -72,45 +74,58 @@ __device__ __forceinline__ float block_max(float x, float* scratch) {
     return s;
 }
 
-// the gradient's factor of a row
-__device__ __forceinline__ float factor_of(const Loss& p, float w, i64 r) {
+// the gradient's factor of a row; den: the sum of the labels' weights
+__device__ __forceinline__ float factor_of(const Loss& p, float w, double den, i64 r) {
     double k = w;
-    if (p.reduction == kMean) k /= *p.den;
+    if (p.reduction == kMean) k /= den;
     if (p.upstream) k *= p.upstream[p.reduction == kNone ? r : 0];
     return (float)k;
 }
 
-// sum of the weights of all labels: parts of the batch, then their sum
+// sum of the weights of all labels, where rows' gradients are to be written before all rows have been seen: at most kWeightParts
+// sums, which every workgroup of the rows' launch adds for itself
+constexpr int kWeightParts = 64;
 __global__ __launch_bounds__(256) void loss_weights_kernel(Loss p) {
     __shared__ double scratch[4];
     double s = 0;
     for (i64 r = (i64)blockIdx.x * 256 + threadIdx.x; r < p.n; r += (i64)gridDim.x * 256) s += weight_of(p, label_at(p, r));
     s = block_sum(s, scratch);
-    if (threadIdx.x == 0) p.part[blockIdx.x] = make_double2(0, s);
+    if (threadIdx.x == 0) p.weight_part[blockIdx.x] = s;
 }
-__global__ __launch_bounds__(256) void loss_join_kernel(Loss p, int weights_only) {
-    __shared__ double scratch[4];
+// in every thread of a wave
+__device__ __forceinline__ double weights_of(const Loss& p) {
+    if (p.weight_parts == 0) return p.den ? *p.den : 1.0;
+    return wave_sum((int)(threadIdx.x & 63) < p.weight_parts ? p.weight_part[threadIdx.x & 63] : 0.0);
+}
+__global__ __launch_bounds__(1024) void loss_join_kernel(Loss p) {
+    __shared__ double scratch[16];
     double a = 0, b = 0;
-    for (int i = threadIdx.x; i < p.parts; i += 256) {
+    for (int i = threadIdx.x; i < p.parts; i += 1024) {
         a += p.part[i].x;
         b += p.part[i].y;
     }
     a = block_sum(a, scratch);
-    b = block_sum(b, scratch);
+    b = p.weight_parts ? weights_of(p) : block_sum(b, scratch);   // what the gradients were made with
     if (threadIdx.x) return;
-    if (weights_only || p.reduction == kMean) *p.den = b;
-    if (!weights_only) *p.loss = (float)(p.reduction == kMean ? a / b : a);
+    if (p.reduction == kMean) *p.den = b;
+    *p.loss = (float)(p.reduction == kMean ? a / b : a);
 }
 
 // ---- few classes: a group of lanes (a power of two, at most 64) per row, E values a lane -----------------------------------
-template <class T, int E, bool BACKWARD>
-__global__ __launch_bounds__(256) void loss_few_kernel(Loss p, int log_lanes) {
-    __shared__ double scratch[4];
+// ONE: a single workgroup takes all rows, and the sums need no other launch
+template <class T, int E, bool BACKWARD, bool ONE>
+__global__ __launch_bounds__(ONE ? 1024 : 256) void loss_few_kernel(Loss p, int log_lanes) {
+    __shared__ double scratch[16];
     const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
-    const i64 r = (i64)blockIdx.x * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
-    double num = 0, den = 0;
+    const i64 groups = blockDim.x >> log_lanes;
+    double num = 0, den = 0, all = 0;
     if (BACKWARD && p.skip_unit && p.reduction != kNone && *p.upstream == 1.0f) return;   // what the forward left is the gradient
-    if (r < p.n) {
+    if (ONE) {
+        for (i64 r = threadIdx.x; r < p.n; r += blockDim.x) all += weight_of(p, label_at(p, r));
+        all = block_sum(all, scratch);
+    } else if (p.grad)
+        all = weights_of(p);
+    for (i64 r = (i64)blockIdx.x * groups + (threadIdx.x >> log_lanes); r < p.n; r += ONE ? groups : p.n) {
         const i64 y = label_at(p, r);
         const float w = weight_of(p, y);
         const T* row = (const T*)p.logits + r * p.stride;
@@ -134,12 +149,11 @@ __global__ __launch_bounds__(256) void loss_few_kernel(Loss p, int log_lanes) {
             p.stat[r] = make_float2(m, z);
             const float l = y != p.ignore ? w * loss_of(m, z, y >= 0 && y < p.c ? to_f32(row[y]) : 0.0f) : 0.0f;
             if (p.reduction == kNone) p.loss[r] = l;
-            num = l;
-            den = w;
+            num += l;
+            den += w;
         }
         if (p.grad) {
-            const float k = factor_of(p, w, r);
-            const float inv = 1.0f / z;
+            const float k = factor_of(p, w, all, r), inv = 1.0f / z;
             T* out = (T*)p.grad + r * p.c;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -150,8 +164,13 @@ __global__ __launch_bounds__(256) void loss_few_kernel(Loss p, int log_lanes) {
     }
     if (BACKWARD || p.reduction == kNone) return;
     num = block_sum(num, scratch);
-    den = block_sum(den, scratch);
-    if (threadIdx.x == 0) p.part[blockIdx.x] = make_double2(num, den);
+    if (!ONE) den = block_sum(den, scratch);
+    if (threadIdx.x) return;
+    if (ONE) {
+        if (p.reduction == kMean) *p.den = all;
+        *p.loss = (float)(p.reduction == kMean ? num / all : num);
+    } else
+        p.part[blockIdx.x] = make_double2(num, den);
 }
 
 // ---- many classes: a workgroup per row -------------------------------------------------------------------------------------
@@ -272,7 +291,7 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
         }
     }
     if (!p.grad) return;
-    const float k = factor_of(p, w, r), inv = 1.0f / z;
+    const float k = factor_of(p, w, weights_of(p), r), inv = 1.0f / z;
     auto gradient = [&](int j, V v) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
@@ -292,12 +311,25 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
 // ---- host -----------------------------------------------------------------------------------------------------------------
 constexpr i64 kFew = 256;   // classes up to which a row is a group of lanes' work
 
+constexpr i64 kOne = 4096;  // lanes' worth of rows up to which one workgroup takes them all: 3 launches less, 4 rows a group at most
+
+int few_lanes(i64 c) {   // 4 values a lane
+    int ll = 0;
+    while ((4 << ll) < c) ++ll;
+    return ll;
+}
+bool one_workgroup(i64 n, i64 c) { return c <= kFew && n << few_lanes(c) <= kOne; }
+
 template <class T, bool BACKWARD> i64 launch_rows(hipStream_t s, const Loss& p) {
     if (p.c <= kFew) {
-        int ll = 0;
-        while ((4 << ll) < p.c) ++ll;   // 4 values a lane
+        const int ll = few_lanes(p.c);
+        if (!BACKWARD && one_workgroup(p.n, p.c)) {
+            const i64 threads = cdiv(p.n << ll, 64) * 64;
+            hipLaunchKernelGGL((loss_few_kernel<T, 4, false, true>), dim3(1), dim3((unsigned)(threads < 1024 ? threads : 1024)), 0, s, p, ll);
+            return 0;
+        }
         const i64 blocks = cdiv(p.n, 256 >> ll);
-        hipLaunchKernelGGL((loss_few_kernel<T, 4, BACKWARD>), dim3((unsigned)blocks), dim3(256), 0, s, p, ll);
+        hipLaunchKernelGGL((loss_few_kernel<T, 4, BACKWARD, false>), dim3((unsigned)blocks), dim3(256), 0, s, p, ll);
         return blocks;
     }
     constexpr int W = 16 / sizeof(T);
@@ -335,14 +367,12 @@ const char* bad_loss(i64 n, i64 c, i64 stride, int dtype, int label_dtype, int r
     if (reduction != kMean && reduction != kSum && reduction != kNone) return "unknown reduction";
     return nullptr;
 }
-constexpr i64 kWeightParts = 256;
-i64 parts_of(i64 n) { return n > kWeightParts ? n : kWeightParts; }
 
 }  // namespace
 
 extern "C" {
 
-int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)(parts_of(n) * sizeof(double2)); }
+int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)(n * sizeof(double2) + kWeightParts * sizeof(double) + 16); }
 
 int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride, const void* labels,
                                   int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction, float* loss, float* stat,
@@ -352,15 +382,16 @@ int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void
     if (!workspace || workspace_bytes < dsp_cross_entropy_workspace(n)) return refuse(who, "workspace too small (dsp_cross_entropy_workspace)");
     if (n && (!logits || !labels || !loss || !stat)) return refuse(who, "NULL pointer");
     if ((reduction != kNone && !loss) || (reduction == kMean && !weight_sum)) return refuse(who, "NULL pointer");
-    Loss p = {logits, labels, weight, grad, loss, (float2*)stat, weight_sum, (double2*)workspace, nullptr, n, c, row_stride, ignore_index, label_dtype, reduction, 0, 0};
+    if ((size_t)workspace & 255) return refuse(who, "the workspace must be aligned to 256 bytes");
+    Loss p = {logits, labels, weight, grad, loss, (float2*)stat, weight_sum, (double2*)workspace, nullptr, n, c, row_stride, ignore_index, label_dtype, reduction, 0, 0,
+              (double*)((double2*)workspace + n), 0};
     hipStream_t s = (hipStream_t)stream;
-    if (grad && reduction == kMean && n) {   // the gradient's factor is known before its rows are
-        p.parts = (int)(cdiv(n, 256) < kWeightParts ? cdiv(n, 256) : kWeightParts);
-        hipLaunchKernelGGL(loss_weights_kernel, dim3(p.parts), dim3(256), 0, s, p);
-        hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(256), 0, s, p, 1);
+    if (grad && reduction == kMean && n && !one_workgroup(n, c)) {
+        p.weight_parts = (int)(cdiv(n, 256) < kWeightParts ? cdiv(n, 256) : kWeightParts);
+        hipLaunchKernelGGL(loss_weights_kernel, dim3(p.weight_parts), dim3(256), 0, s, p);
     }
     p.parts = n ? (int)launch_typed<false>(s, p, dtype) : 0;
-    if (reduction != kNone) hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(256), 0, s, p, 0);
+    if (reduction != kNone && (n == 0 || !one_workgroup(n, c))) hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(1024), 0, s, p);
     return launched(who);
 }
 
@@ -372,7 +403,7 @@ int32_t dsp_cross_entropy_backward(void* stream, int64_t n, int64_t c, const voi
     if (n == 0) return DSP_OK;
     if (!logits || !labels || !stat || !upstream || !grad || (reduction == kMean && !weight_sum)) return refuse(who, "NULL pointer");
     Loss p = {logits, labels, weight, grad, nullptr, (float2*)stat, (double*)weight_sum, nullptr, upstream, n, c, row_stride, ignore_index, label_dtype,
-              reduction, 0, skip_unit};
+              reduction, 0, skip_unit, nullptr, 0};
     launch_typed<true>((hipStream_t)stream, p, dtype);
     return launched(who);
 }

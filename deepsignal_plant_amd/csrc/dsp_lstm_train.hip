@@ -12,74 +12,76 @@
 // behind it) is done by one product over all steps; the recurrence is a launch per step for both directions, its product,
 // the gates and the states in one kernel.  A launch ends before the next begins, so no workgroup waits for another.
 //
-// Layouts: x [B][T][I], y [B][T][dirs H], states [dirs][B][H], gates [dirs][T][B][4H] and cells [dirs][T][B][H] by the time in
-// the sequence; a row of the products over all steps is m = t B + b.
+// Layouts: x [B][T][I], y [B][T][dirs H], states [dirs][B][H]; gates and their gradients [dirs][B][T][4H]; cells and the h before
+// each step [dirs][B][T][H].  So the products over all steps are plain: a row is m = b T + t.
 #include "dsp_ops.h"
 
 using namespace dsp;
 
 namespace {
 
-// ---- operands of a product C(m, n) = sum over k of A(m, k) B(n, k) -------------------------------------------------------
-// kAlongK: values of a row lie along k (at(row) + k);  otherwise along the rows (at(k) + row).  NULL: zeros.
-struct Plain {   // rows (or columns) `ld` apart
-    const float* p[2];
-    i64 ld;
-    __device__ __forceinline__ const float* at(int d, int i) const { return p[d] + i * ld; }
-};
-struct Inputs {   // x by m = t B + b
-    const float* x;
-    int B, T, I;
-    __device__ __forceinline__ const float* at(int, int m) const {
-        const int t = m / B, b = m - t * B;
-        return x + ((i64)b * T + t) * I;
-    }
-};
-struct Before {   // h of the step before, by m = t B + b
-    const float *y, *h0;
-    int B, T, H, dirs;
-    __device__ __forceinline__ const float* at(int d, int m) const {
-        const int t = m / B, b = m - t * B, before = d ? t + 1 : t - 1;
-        if (before < 0 || before >= T) return h0 ? h0 + ((i64)d * B + b) * H : nullptr;
-        return y + (((i64)b * T + before) * dirs + d) * H;
-    }
-};
-
-// ---- the product over all steps --------------------------------------------------------------------------------------------
-// A workgroup of 4 waves makes a tile of TILE x TILE, a wave a quarter of it as 32 x 32 blocks of v_mfma_f32_32x32x2; 16 values
-// of k are staged in LDS at a time, the next 16 on their way in registers meanwhile.  A lane's 4 values of k are consecutive
-// (lane group q: k = 4q + j for instruction j): the order of k is the same for both operands, so any is right.
+// ---- the products over all steps -----------------------------------------------------------------------------------------
+// C(m, n) = sum over k of A(m, k) B(n, k).  A workgroup of 4 waves makes a tile of TILE x TILE, a wave a quarter of it as 32 x 32
+// blocks of v_mfma_f32_32x32x2.  16 values of k are staged in LDS at a time, the next 16 on their way in registers and the ones
+// before them in the other half of LDS: one barrier per 16.  A lane's 4 values of k are consecutive (lane group q takes k =
+// 4q + j for instruction j): the order of k is the same for both operands, so any is right.
+//
+// On this device vector instructions take their time from the fp32 matrix instructions, so the loop has next to none: where
+// sizes and addresses allow (FAST), the operands come by buffer loads whose lane offsets are made once and whose descriptors
+// end with the operand: what lies behind it reads as zeros.  Otherwise (an input size of 7) every value is guarded.
 constexpr int kStep = 16;
 
-template <bool ALONG_K, int TILE> struct Stage {
+struct Matrix {   // row-major, `lines` lines of `ld` values
+    const float* p;
+    int lines, ld;
+};
+
+// ALONG_K: a line is a row of the product, k along it.  Else a line is a k, the product's rows along it.
+template <bool ALONG_K, int TILE, bool FAST> struct Stage {
     static constexpr int kStride = ALONG_K ? kStep + 4 : TILE + 4;
     static constexpr int kFloats = ALONG_K ? TILE * kStride : kStep * kStride;
-    static constexpr int kLoads = TILE * kStep / 4 / 256;
+    static constexpr int kLoads = TILE * kStep / 4 / 256, kAcross = ALONG_K ? kStep / 4 : TILE / 4;   // accesses of 4 along a line
     f32x4 v[kLoads];
-    // `rows`, `k_end`: bounds of the operand; row0, k0: the tile's
-    template <class Op> __device__ __forceinline__ void fetch(const Op& op, int d, int row0, int rows, int k0, int k_end, bool wide) {
+    Matrix m;
+    int row0, k_end;
+    __amdgpu_buffer_rsrc_t rsrc;
+    int lane_at[kLoads];
+    uint32_t at, per_step;
+    __device__ __forceinline__ Stage(const Matrix& matrix, int row, int k0, int k1) : m(matrix), row0(row), k_end(k1) {
+        if (!FAST) return;
+        const float* base = ALONG_K ? m.p + (i64)row0 * m.ld : m.p + (i64)k0 * m.ld + row0;
+        const i64 bytes = ((i64)m.lines * m.ld - (base - m.p)) * 4;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes), 0x00020000);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int j = threadIdx.x + i * 256;
-            const int a = ALONG_K ? row0 + j / (kStep / 4) : k0 + j / (TILE / 4);                     // which line
-            const int b = ALONG_K ? k0 + j % (kStep / 4) * 4 : row0 + j % (TILE / 4) * 4;             // where on it
-            const int lines = ALONG_K ? rows : k_end, most = ALONG_K ? k_end : rows;
-            v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const float* p = a < lines ? op.at(d, a) : nullptr;
-            if (!p) continue;
-            if (wide && b + 4 <= most) v[i] = *(const f32x4*)(p + b);
-            else
+            lane_at[i] = (j / kAcross * m.ld + j % kAcross * 4) * 4;
+        }
+        at = ALONG_K ? k0 * 4 : 0;
+        per_step = ALONG_K ? kStep * 4 : (uint32_t)m.ld * kStep * 4;
+    }
+    __device__ __forceinline__ void fetch(int k) {
+        if (FAST) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (b + e < most) v[i][e] = p[b + e];
+            for (int i = 0; i < kLoads; ++i) v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane_at[i], (int)at, 0));
+            at += per_step;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int j = threadIdx.x + i * 256;
+            const int line = (ALONG_K ? row0 : k) + j / kAcross, on = (ALONG_K ? k : row0) + j % kAcross * 4;
+            const int lines = ALONG_K ? m.lines : k_end, most = ALONG_K ? k_end : m.ld;
+            const float* p = m.p + (i64)line * m.ld + on;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = line < lines && on + e < most ? p[e] : 0.0f;
         }
     }
     __device__ __forceinline__ void put(float* lds) const {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int j = threadIdx.x + i * 256;
-            const int at = ALONG_K ? j / (kStep / 4) * kStride + j % (kStep / 4) * 4 : j / (TILE / 4) * kStride + j % (TILE / 4) * 4;
-            *(f32x4*)(lds + at) = v[i];
+            *(f32x4*)(lds + j / kAcross * kStride + j % kAcross * 4) = v[i];
         }
     }
     // 4 consecutive values of k of one row
@@ -91,30 +93,23 @@ template <bool ALONG_K, int TILE> struct Stage {
         return r;
     }
 };
+template <bool A_ALONG_K, bool B_ALONG_K, int TILE> constexpr int half_floats() {
+    return Stage<A_ALONG_K, TILE, false>::kFloats + Stage<B_ALONG_K, TILE, false>::kFloats;
+}
 
-// C tile += over k in [k0, k1) of direction d;  acc[i][j]: block (i, j) of the wave's quarter
-template <bool A_ALONG_K, bool B_ALONG_K, int TILE, class A, class B>
-__device__ __forceinline__ void product(const A& a, const B& b, int d, int m0, int M, int n0, int N, int k0, int k1, bool wide_a, bool wide_b,
-                                        float* lds, f32x16 (&acc)[TILE / 64][TILE / 64]) {
-    typedef Stage<A_ALONG_K, TILE> SA;
-    typedef Stage<B_ALONG_K, TILE> SB;
-    constexpr int R = TILE / 64;
-    float *la = lds, *lb = lds + SA::kFloats;
+// acc[i][j] (block (i, j) of the wave's quarter) += over k in [k0, k1).  f(values of A as they are staged) for every 16 of k
+template <bool A_ALONG_K, bool B_ALONG_K, int TILE, bool FAST, class F>
+__device__ __forceinline__ void product(const Matrix& a, const Matrix& b, int m0, int n0, int k0, int k1, float* lds, f32x16 (&acc)[TILE / 64][TILE / 64], F f) {
+    typedef Stage<A_ALONG_K, TILE, FAST> SA;
+    typedef Stage<B_ALONG_K, TILE, FAST> SB;
+    constexpr int R = TILE / 64, HALF = SA::kFloats + SB::kFloats;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = (wave >> 1) * (TILE / 2) + (lane & 31), wn = (wave & 1) * (TILE / 2) + (lane & 31), kq = (lane >> 5) * 4;
-    SA sa;
-    SB sb;
-    sa.fetch(a, d, m0, M, k0, k1, wide_a);
-    sb.fetch(b, d, n0, N, k0, k1, wide_b);
-    for (int k = k0; k < k1; k += kStep) {
-        __syncthreads();
-        sa.put(la);
-        sb.put(lb);
-        __syncthreads();
-        if (k + kStep < k1) {
-            sa.fetch(a, d, m0, M, k + kStep, k1, wide_a);
-            sb.fetch(b, d, n0, N, k + kStep, k1, wide_b);
-        }
+    if (k0 >= k1) return;
+    SA sa(a, m0, k0, k1);
+    SB sb(b, n0, k0, k1);
+    auto step = [&](int half, int k) {   // 16 values of k from one half of LDS; the next 16 into the other
+        const float *la = lds + half * HALF, *lb = la + SA::kFloats;
 #pragma unroll
         for (int kk = 0; kk < kStep; kk += 8) {
             f32x4 fa[R], fb[R];
@@ -130,6 +125,32 @@ __device__ __forceinline__ void product(const A& a, const B& b, int d, int m0, i
 #pragma unroll
                     for (int j = 0; j < R; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
         }
+        if (k + kStep < k1) {
+            float* next = lds + (half ^ 1) * HALF;
+            f(sa.v);
+            sa.put(next);
+            sb.put(next + SA::kFloats);
+            if (k + 2 * kStep < k1) {
+                sa.fetch(k + 2 * kStep);
+                sb.fetch(k + 2 * kStep);
+            }
+        }
+        __syncthreads();
+    };
+    sa.fetch(k0);
+    sb.fetch(k0);
+    __syncthreads();   // what used LDS before is done
+    f(sa.v);
+    sa.put(lds);
+    sb.put(lds + SA::kFloats);
+    if (k0 + kStep < k1) {
+        sa.fetch(k0 + kStep);
+        sb.fetch(k0 + kStep);
+    }
+    __syncthreads();
+    for (int k = k0; k < k1; k += 2 * kStep) {
+        step(0, k);
+        if (k + kStep < k1) step(1, k + kStep);
     }
 }
 // f(m, n, value) for every value of the tile that is inside
@@ -146,97 +167,95 @@ template <int TILE, class F> __device__ __forceinline__ void each(const f32x16 (
                 if (m < M && n < N) f(m, n, acc[i][j][r]);
             }
 }
-template <bool A_ALONG_K, bool B_ALONG_K, int TILE> constexpr int lds_floats() { return Stage<A_ALONG_K, TILE>::kFloats + Stage<B_ALONG_K, TILE>::kFloats; }
+// Workgroups go to the 8 dies in turn, each with an L2 of its own: give each die a contiguous range of the tiles, so that tiles of the same
+// rows (neighbours in it) find them there.
+__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint32_t tiles) {
+    const uint32_t die = block & 7, per = tiles >> 3, more = tiles & 7;
+    return die * per + (die < more ? die : more) + (block >> 3);
+}
+struct Nothing { template <class V> __device__ __forceinline__ void operator()(const V&) const {} };
 
-struct Shape { int B, T, I, H, dirs, wide_x, wide_h, wide_wx; };   // wide_*: accesses of 16 bytes along I of x, along H, along I of W_ih
+struct Shape { int B, T, I, H, dirs; };
 struct Weights { const float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
 
-// gates = W_ih x + b_ih + b_hh, all steps;  blockIdx.z: direction
-template <int TILE> __global__ __launch_bounds__(256) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
-    __shared__ __attribute__((aligned(16))) float lds[lds_floats<true, true, TILE>()];
-    const int d = blockIdx.z, m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, M = s.B * s.T, N = 4 * s.H;
-    const Inputs a = {x, s.B, s.T, s.I};
-    const Plain b = {{w.w_ih[0], w.w_ih[1]}, s.I};
+// gates = W_ih x + b_ih + b_hh, all steps
+template <int TILE, bool FAST> __global__ __launch_bounds__(256) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, TILE>()];
+    const int M = s.B * s.T, N = 4 * s.H, n_tiles = (N + TILE - 1) / TILE;
+    const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const int n0 = tile % (n_tiles * s.dirs), d = n0 / n_tiles, at = (n0 - d * n_tiles) * TILE, m0 = tile / (n_tiles * s.dirs) * TILE;
     f32x16 acc[TILE / 64][TILE / 64] = {};
-    product<true, true, TILE>(a, b, d, m0, M, n0, N, 0, s.I, s.wide_x, s.wide_wx, lds, acc);
+    product<true, true, TILE, FAST>({x, M, s.I}, {w.w_ih[d], N, s.I}, m0, at, 0, s.I, lds, acc, Nothing());
     float* out = gates + (i64)d * M * N;
-    each<TILE>(acc, m0, M, n0, N, [&](int m, int n, float v) { out[(i64)m * N + n] = v + (w.b_ih[d][n] + w.b_hh[d][n]); });
+    each<TILE>(acc, m0, M, at, N, [&](int m, int n, float v) { out[(i64)m * N + n] = v + (w.b_ih[d][n] + w.b_hh[d][n]); });
 }
 
 // dx = sum over directions of dz W_ih
-template <int TILE> __global__ __launch_bounds__(256) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
-    __shared__ __attribute__((aligned(16))) float lds[lds_floats<true, false, TILE>()];
-    const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, M = s.B * s.T, K = 4 * s.H;
-    const Plain a = {{dz, dz + (i64)M * K}, K}, b = {{w.w_ih[0], w.w_ih[1]}, s.I};
+template <int TILE, bool FAST> __global__ __launch_bounds__(256) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, false, TILE>()];
+    const int M = s.B * s.T, K = 4 * s.H, n_tiles = (s.I + TILE - 1) / TILE;
+    const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const int n0 = tile % n_tiles * TILE, m0 = tile / n_tiles * TILE;
     f32x16 acc[TILE / 64][TILE / 64] = {};
-    for (int d = 0; d < s.dirs; ++d) product<true, false, TILE>(a, b, d, m0, M, n0, s.I, 0, K, true, s.wide_wx, lds, acc);
-    each<TILE>(acc, m0, M, n0, s.I, [&](int m, int n, float v) {
-        const int t = m / s.B, b = m - t * s.B;
-        dx[((i64)b * s.T + t) * s.I + n] = v;
-    });
+    for (int d = 0; d < s.dirs; ++d)
+        product<true, false, TILE, FAST>({dz + (i64)d * M * K, M, K}, {w.w_ih[d], K, s.I}, m0, n0, 0, K, lds, acc, Nothing());
+    each<TILE>(acc, m0, M, n0, s.I, [&](int m, int n, float v) { dx[(i64)m * s.I + n] = v; });
 }
 
-// dW of both weights: tiles of [4H][I] first, tiles of [4H][H] behind them; blockIdx.z = direction x part of the sum over m.  Where
-// there is one part it writes the gradients, else part[part][direction][4H][I + H] for lstm_join_kernel.
-template <int TILE>
-__global__ __launch_bounds__(256) void lstm_weight_grad_kernel(Shape s, const float* __restrict__ dz, const float* __restrict__ x, const float* __restrict__ y,
-                                                               const float* __restrict__ h0, int parts, int per_part, int x_tiles, float* __restrict__ part,
-                                                               float* dw_ih0, float* dw_ih1, float* dw_hh0, float* dw_hh1) {
-    __shared__ __attribute__((aligned(16))) float lds[lds_floats<false, false, TILE>()];
-    const int d = blockIdx.z / parts, q = blockIdx.z - d * parts, m0 = blockIdx.y * TILE, M = 4 * s.H, K = s.B * s.T;
-    const bool of_x = (int)blockIdx.x < x_tiles;
-    const int n0 = (of_x ? blockIdx.x : blockIdx.x - x_tiles) * TILE, N = of_x ? s.I : s.H;
+// dW of both weights and db: tiles of [4H][I] and [4H][H], the sum over m in parts;  part [parts][dirs][4H][I + H + 1]
+template <int TILE, bool FAST>
+__global__ __launch_bounds__(256) void lstm_weight_grad_kernel(Shape s, const float* __restrict__ dz, const float* __restrict__ x, const float* __restrict__ h_before,
+                                                               int per_part, float* __restrict__ part) {
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<false, false, TILE>()];
+    const int M = 4 * s.H, K = s.B * s.T, m_tiles = (M + TILE - 1) / TILE, x_tiles = (s.I + TILE - 1) / TILE, n_tiles = x_tiles + (s.H + TILE - 1) / TILE;
+    uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const int nt = tile % n_tiles;
+    tile /= n_tiles;
+    const int m0 = tile % m_tiles * TILE, dq = tile / m_tiles, d = dq % s.dirs, q = dq / s.dirs;
+    const bool of_x = nt < x_tiles;
+    const int n0 = (of_x ? nt : nt - x_tiles) * TILE, N = of_x ? s.I : s.H, cols = s.I + s.H + 1;
     const int k0 = q * per_part, k1 = k0 + per_part < K ? k0 + per_part : K;
-    const Plain a = {{dz, dz + (i64)M * K}, M};
+    const Matrix a = {dz + (i64)d * K * M, K, M}, b = {of_x ? x : h_before + (i64)d * K * s.H, K, N};
     f32x16 acc[TILE / 64][TILE / 64] = {};
-    if (of_x) {
-        const Inputs b = {x, s.B, s.T, s.I};
-        product<false, false, TILE>(a, b, d, m0, M, n0, N, k0, k1, true, s.wide_x, lds, acc);
-    } else {
-        const Before b = {y, h0, s.B, s.T, s.H, s.dirs};
-        product<false, false, TILE>(a, b, d, m0, M, n0, N, k0, k1, true, s.wide_h, lds, acc);
-    }
-    if (parts == 1) {
-        float* out = of_x ? (d ? dw_ih1 : dw_ih0) : (d ? dw_hh1 : dw_hh0);
-        each<TILE>(acc, m0, M, n0, N, [&](int m, int n, float v) { out[(i64)m * N + n] = v; });
-    } else {
-        float* out = part + ((i64)q * s.dirs + d) * M * (s.I + s.H) + (of_x ? 0 : s.I);
-        each<TILE>(acc, m0, M, n0, N, [&](int m, int n, float v) { out[(i64)m * (s.I + s.H) + n] = v; });
-    }
+    float* out = part + (i64)dq * M * cols;
+    if (nt == 0) {   // these see every dz of their rows once: db on the way
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        product<false, false, TILE, FAST>(a, b, m0, n0, k0, k1, lds, acc, [&](const auto& v) {
+            for (const f32x4& y : v) sum += y;
+        });
+        // a thread has summed 4 rows for the values of k that came to it: rows by access along a line, k by line
+        constexpr int kAcross = TILE / 4, kLines = 256 / kAcross;
+        f32x4* sums = (f32x4*)lds;
+        __syncthreads();
+        sums[threadIdx.x] = sum;
+        __syncthreads();
+        if (threadIdx.x < kAcross) {
+            for (int i = 1; i < kLines; ++i) sum += sums[i * kAcross + threadIdx.x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (m0 + (int)threadIdx.x * 4 + e < M) out[(i64)(m0 + threadIdx.x * 4 + e) * cols + cols - 1] = sum[e];
+        }
+    } else
+        product<false, false, TILE, FAST>(a, b, m0, n0, k0, k1, lds, acc, Nothing());
+    each<TILE>(acc, m0, M, n0, N, [&](int m, int n, float v) { out[(i64)m * cols + n + (of_x ? 0 : s.I)] = v; });
 }
-// the parts in order, and both weights apart
-__global__ __launch_bounds__(256) void lstm_join_kernel(Shape s, int parts, const float* __restrict__ part, float* dw_ih0, float* dw_ih1, float* dw_hh0, float* dw_hh1) {
-    const i64 one = (i64)4 * s.H * (s.I + s.H), i = (i64)blockIdx.x * 256 + threadIdx.x;
+struct Grads { float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
+// the parts in order, and the gradients apart
+__global__ __launch_bounds__(256) void lstm_join_kernel(Shape s, int parts, const float* __restrict__ part, Grads g) {
+    const int cols = s.I + s.H + 1;
+    const i64 one = (i64)4 * s.H * cols, i = (i64)blockIdx.x * 256 + threadIdx.x;
     if (i >= one * s.dirs) return;
     float v = 0.0f;
     for (int q = 0; q < parts; ++q) v += part[q * one * s.dirs + i];
     const int d = i >= one;
-    const i64 j = i - d * one, m = j / (s.I + s.H);
-    const int n = (int)(j - m * (s.I + s.H));
-    if (n < s.I) (d ? dw_ih1 : dw_ih0)[m * s.I + n] = v;
-    else (d ? dw_hh1 : dw_hh0)[m * s.H + n - s.I] = v;
-}
-
-// db: sums of dz over m.  64 columns a workgroup, a quarter of its rows a wave; part[rows of workgroups][dirs][4H]
-__global__ __launch_bounds__(256) void lstm_bias_grad_kernel(Shape s, const float* __restrict__ dz, int per_part, float* __restrict__ part) {
-    __shared__ float sums[4][64];
-    const int d = blockIdx.z, M = s.B * s.T, N = 4 * s.H, n = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    const int from = blockIdx.y * per_part, to = from + per_part < M ? from + per_part : M;
-    float v = 0.0f;
-    if (n < N)
-        for (int m = from + q; m < to; m += 4) v += dz[((i64)d * M + m) * N + n];
-    sums[q][threadIdx.x & 63] = v;
-    __syncthreads();
-    if (q == 0 && n < N) part[((i64)blockIdx.y * s.dirs + d) * N + n] = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
-}
-__global__ __launch_bounds__(256) void lstm_bias_join_kernel(Shape s, int parts, const float* __restrict__ part, float* db0, float* db1, float* db2, float* db3) {
-    const int N = 4 * s.H, i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * s.dirs) return;
-    float v = 0.0f;
-    for (int q = 0; q < parts; ++q) v += part[(i64)q * N * s.dirs + i];
-    const int d = i >= N, n = i - d * N;
-    (d ? db1 : db0)[n] = v;   // b_ih and b_hh are added to the same place
-    (d ? db3 : db2)[n] = v;
+    const i64 j = i - d * one, m = j / cols;
+    const int n = (int)(j - m * cols);
+    if (n < s.I) g.w_ih[d][m * s.I + n] = v;
+    else if (n < s.I + s.H) g.w_hh[d][m * s.H + n - s.I] = v;
+    else {
+        g.b_ih[d][m] = v;   // both biases are added to the same place
+        g.b_hh[d][m] = v;
+    }
 }
 
 // ---- the recurrence ----------------------------------------------------------------------------------------------------------
@@ -253,114 +272,149 @@ __device__ __forceinline__ float tanh_of(float x) {
     return copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e), x);
 }
 
-// A workgroup's tile: 64 sequences by 16 columns of each of G groups of columns (forward: the 4 gates of 16 units; backward:
-// 16 units); a wave takes 16 sequences.  acc[g] += A [64][K] (rows by `row`, NULL = zeros) x W [columns][K], values along k in both,
-// 32 values of k staged in LDS at a time.
-constexpr int kSeqs = 64, kUnits = 16, kDepth = 32, kPad = kDepth + 4;
-
-template <int G, class Row, class Col>
-__device__ __forceinline__ void step_product(int K, bool wide, Row row, Col col, float* lds, f32x4 (&acc)[G]) {
-    float *la = lds, *lw = lds + kSeqs * kPad;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int LA = kSeqs * kDepth / 4 / 256, LW = (G * kUnits * kDepth / 4 + 255) / 256;
-    f32x4 va[LA], vw[LW];
+// A workgroup of 4 waves makes a tile of 16 S sequences by C blocks of 16 columns (forward: the 4 gates of 16 units; backward: 16 units).
+// Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves: it goes from memory straight into
+// the registers in which v_mfma_f32_16x16x4 takes it (4 consecutive k a lane, as above), without LDS and barriers, D accesses ahead.
+// The quarters are joined through LDS at the end, in order.  WIDE: k comes in whole accesses of 4 and steps of 16.
+// a[i], w[i]: the lane's row of the i-th 16 rows.  Rows behind the last are clamped to it: what they give is not used.
+template <int S, int C, int D, bool WIDE> __device__ __forceinline__ void step_product(int K, const float* const (&a)[S], const float* const (&w)[C], f32x4 (&acc)[C][S]) {
+    const int q = (threadIdx.x & 63) >> 4, wave = threadIdx.x >> 6;
+    const int steps = (K + 15) >> 4, per = (steps + 3) >> 2, from = wave * per, to = from + per < steps ? from + per : steps;
+    f32x4 fa[D][S], fw[D][C];
     auto load = [&](const float* p, int k) {
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (!p) return v;
-        if (wide && k + 4 <= K) return *(const f32x4*)(p + k);
+        if (WIDE) return *(const f32x4*)(p + k);
+        f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (k + e < K) v[e] = p[k + e];
+        for (int e = 0; e < 4; ++e) v[e] = k + e < K ? p[k + e] : 0.0f;
         return v;
     };
-    auto fetch = [&](int k) {
+    auto fetch = [&](int i, int step) {
 #pragma unroll
-        for (int i = 0; i < LA; ++i) {
-            const int j = threadIdx.x + i * 256;
-            va[i] = load(row(j / (kDepth / 4)), k + j % (kDepth / 4) * 4);
-        }
+        for (int j = 0; j < S; ++j) fa[i][j] = load(a[j], step * 16 + q * 4);
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            const int j = threadIdx.x + i * 256;
-            if (j < G * kUnits * kDepth / 4) vw[i] = load(col(j / (kDepth / 4)), k + j % (kDepth / 4) * 4);
-        }
+        for (int j = 0; j < C; ++j) fw[i][j] = load(w[j], step * 16 + q * 4);
     };
-    fetch(0);
-    for (int k = 0; k < K; k += kDepth) {
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < LA; ++i) {
-            const int j = threadIdx.x + i * 256;
-            *(f32x4*)(la + j / (kDepth / 4) * kPad + j % (kDepth / 4) * 4) = va[i];
-        }
+    for (int i = 0; i < D; ++i)
+        if (from + i < to) fetch(i, from + i);
+    for (int step = from; step < to; step += D)
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            const int j = threadIdx.x + i * 256;
-            if (j < G * kUnits * kDepth / 4) *(f32x4*)(lw + j / (kDepth / 4) * kPad + j % (kDepth / 4) * 4) = vw[i];
-        }
-        __syncthreads();
-        if (k + kDepth < K) fetch(k + kDepth);
-#pragma unroll
-        for (int kk = 0; kk < kDepth; kk += 16) {
-            const int at = kk + (lane >> 4) * 4;
-            const f32x4 a = *(const f32x4*)(la + (wave * 16 + (lane & 15)) * kPad + at);
-            f32x4 w[G];
-#pragma unroll
-            for (int g = 0; g < G; ++g) w[g] = *(const f32x4*)(lw + (g * kUnits + (lane & 15)) * kPad + at);
+        for (int i = 0; i < D; ++i) {
+            if (step + i >= to) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int g = 0; g < G; ++g) acc[g] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], w[g][e], acc[g], 0, 0, 0);
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i][j][e], fw[i][c][e], acc[c][j], 0, 0, 0);
+            if (step + i + D < to) fetch(i, step + i + D);
         }
-    }
+}
+// the sums of the 4 waves: f(c, row, unit, value) -- of every value of the tile, a thread's rows 16 apart
+constexpr int kRow = 17;   // floats of a row of 16 in LDS
+template <int S, int C> constexpr int step_floats() { return 4 * C * S * 16 * kRow; }
+template <int S, int C> __device__ __forceinline__ void step_join(const f32x4 (&acc)[C][S], float* lds, float (&sum)[S][C]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[((wave * C + c) * S * 16 + j * 16 + (lane >> 4) * 4 + r) * kRow + (lane & 15)] = acc[c][j][r];
+    __syncthreads();
+    const int row = threadIdx.x >> 4, unit = threadIdx.x & 15;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            sum[j][c] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[j][c] += lds[((v * C + c) * S * 16 + j * 16 + row) * kRow + unit];
+        }
+}
+// 16 units fastest, then sequences, then direction, a contiguous range for each die: with two directions it sees one of them, the states
+// of its own sequences and whole lines of their gates
+struct Place { int d, u0, b0; };
+template <int S> __device__ __forceinline__ Place place_of(const Shape& s) {
+    const uint32_t units = (s.H + 15) >> 4, seqs = (s.B + 16 * S - 1) / (16 * S);
+    uint32_t i = tile_of(blockIdx.x, gridDim.x);
+    Place p;
+    p.u0 = i % units * 16;
+    i /= units;
+    p.b0 = i % seqs * (16 * S);
+    p.d = i / seqs;
+    return p;
 }
 
-// gates: in W_ih x + b of all steps; out (save) i, f, g, o.  cells: c of all steps (save), else of two steps in turn
-__global__ __launch_bounds__(256) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ h0, const float* __restrict__ c0,
-                                                        float* gates, float* cells, float* y, float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ __attribute__((aligned(16))) float lds[(kSeqs + 4 * kUnits) * kPad];
-    const int d = blockIdx.z, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1;
-    const int b0 = blockIdx.x * kSeqs, u0 = blockIdx.y * kUnits;
-    f32x4 acc[4] = {};
-    if (step > 0 || h0) {
-        const float* w_hh = w.w_hh[d];
-        step_product<4>(
-            H, s.wide_h,
-            [&](int i) -> const float* {
-                const int b = b0 + i;
-                if (b >= B) return nullptr;
-                return step ? y + (((i64)b * T + before) * s.dirs + d) * H : h0 + ((i64)d * B + b) * H;
-            },
-            [&](int j) -> const float* {
-                const int u = u0 + j % kUnits;
-                return u < H ? w_hh + ((i64)(j / kUnits) * H + u) * H : nullptr;
-            },
-            lds, acc);
+// gates: in W_ih x + b of all steps (FUSED: made here, from x); out (save) i, f, g, o.  cells: c of all steps (save), else of two steps
+// in turn; h_before (save): h before each step
+template <int S, bool WIDE, bool FUSED>
+__global__ __launch_bounds__(256) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ x, const float* __restrict__ h0,
+                                                        const float* __restrict__ c0, float* gates, float* cells, float* h_before, float* y,
+                                                        float* __restrict__ hn, float* __restrict__ cn, int save) {
+    __shared__ float lds[step_floats<S, 4>()];
+    const Place p = place_of<S>(s);
+    const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15);
+    // what the gates need besides, on its way meanwhile
+    float z[S][4], c[S];
+    const int uc = u < H ? u : H - 1;
+    i64 at[S], m[S];
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+        const int b = p.b0 + j * 16 + row < B ? p.b0 + j * 16 + row : B - 1;
+        at[j] = ((i64)d * B + b) * H + uc;
+        m[j] = ((i64)d * B + b) * T + t;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) z[j][g] = FUSED ? w.b_ih[d][g * H + uc] + w.b_hh[d][g * H + uc] : gates[m[j] * 4 * H + g * H + uc];
+        c[j] = 0.0f;
+        if (step) c[j] = save ? cells[(m[j] + before - t) * H + uc] : cells[((step - 1) & 1) * (i64)s.dirs * B * H + at[j]];
+        else if (c0) c[j] = c0[at[j]];
     }
-    const int lane = threadIdx.x & 63, u = u0 + (lane & 15);
+    f32x4 acc[4][S] = {};
+    const float *a[S], *v[4];
+    const int wu = p.u0 + (lane & 15) < H ? p.u0 + (lane & 15) : H - 1;
+    if (FUSED) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) a[j] = x + ((i64)(p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1) * T + t) * s.I;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) v[g] = w.w_ih[d] + ((i64)g * H + wu) * s.I;
+        step_product<S, 4, 2, WIDE>(s.I, a, v, acc);
+    }
+    if (step > 0 || h0) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const i64 b = p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1;
+            a[j] = step ? y + ((b * T + before) * s.dirs + d) * H : h0 + ((i64)d * B + b) * H;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) v[g] = w.w_hh[d] + ((i64)g * H + wu) * H;
+        step_product<S, 4, 2, WIDE>(H, a, v, acc);
+    }
+    float sum[S][4];
+    step_join<S, 4>(acc, lds, sum);
     if (u >= H) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int b = b0 + (threadIdx.x >> 6) * 16 + (lane >> 4) * 4 + r;
+    for (int j = 0; j < S; ++j) {
+        const i64 b = p.b0 + j * 16 + row;
         if (b >= B) continue;
-        float* z = gates + (((i64)d * T + t) * B + b) * 4 * H + u;
-        const float i = sigmoid(z[0] + acc[0][r]), f = sigmoid(z[H] + acc[1][r]), g = tanh_of(z[2 * H] + acc[2][r]), o = sigmoid(z[3 * H] + acc[3][r]);
-        float c = 0.0f;
-        if (step) c = cells[(((i64)d * (save ? T : 2) + (save ? before : (step - 1) & 1)) * B + b) * H + u];
-        else if (c0) c = c0[((i64)d * B + b) * H + u];
-        c = f * c + i * g;
-        const float h = o * tanh_of(c);
+        const float i = sigmoid(z[j][0] + sum[j][0]), f = sigmoid(z[j][1] + sum[j][1]), g = tanh_of(z[j][2] + sum[j][2]), o = sigmoid(z[j][3] + sum[j][3]);
+        const float cell = f * c[j] + i * g, h = o * tanh_of(cell);
         if (save) {
-            z[0] = i;
-            z[H] = f;
-            z[2 * H] = g;
-            z[3 * H] = o;
-        }
-        cells[(((i64)d * (save ? T : 2) + (save ? t : step & 1)) * B + b) * H + u] = c;
-        y[(((i64)b * T + t) * s.dirs + d) * H + u] = h;
+            float* q = gates + m[j] * 4 * H + u;
+            q[0] = i;
+            q[H] = f;
+            q[2 * H] = g;
+            q[3 * H] = o;
+            cells[m[j] * H + u] = cell;
+            if (step == 0) h_before[m[j] * H + u] = h0 ? h0[at[j]] : 0.0f;
+            if (step < T - 1) h_before[(m[j] + after - t) * H + u] = h;
+        } else
+            cells[(step & 1) * (i64)s.dirs * B * H + at[j]] = cell;
+        y[((b * T + t) * s.dirs + d) * H + u] = h;
         if (step == T - 1) {
-            hn[((i64)d * B + b) * H + u] = h;
-            cn[((i64)d * B + b) * H + u] = c;
+            hn[at[j]] = h;
+            cn[at[j]] = cell;
         }
     }
 }
@@ -377,47 +431,58 @@ __global__ __launch_bounds__(256) void lstm_transpose_kernel(int H, Weights w, f
 }
 
 // One step back; step = T - 1 .. 0, and -1 for the gradient of h0.  dc: gradient of the cell between steps, of c0 in the end.
+template <int S, bool WIDE>
 __global__ __launch_bounds__(256) void lstm_step_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0,
                                                              const float* __restrict__ gates, const float* __restrict__ cells, const float* __restrict__ gy,
                                                              const float* __restrict__ ghn, const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
-    __shared__ __attribute__((aligned(16))) float lds[(kSeqs + kUnits) * kPad];
-    const int d = blockIdx.z, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
-    const int b0 = blockIdx.x * kSeqs, u0 = blockIdx.y * kUnits;
-    f32x4 acc[1] = {};
-    if (step < T - 1)
-        step_product<1>(
-            4 * H, true,
-            [&](int i) -> const float* {
-                const int b = b0 + i;
-                return b < B ? dz + (((i64)d * T + after) * B + b) * 4 * H : nullptr;
-            },
-            [&](int j) -> const float* { return u0 + j < H ? w_hh_t + ((i64)d * H + u0 + j) * 4 * H : nullptr; }, lds, acc);
-    const int lane = threadIdx.x & 63, u = u0 + (lane & 15);
+    __shared__ float lds[step_floats<S, 1>()];
+    const Place p = place_of<S>(s);
+    const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15), uc = u < H ? u : H - 1;
+    float gate[S][4], c[S], c_before[S], dct[S], dh[S];
+    i64 at[S], m[S];
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+        const i64 b = p.b0 + j * 16 + row < B ? p.b0 + j * 16 + row : B - 1;
+        at[j] = ((i64)d * B + b) * H + uc;
+        m[j] = ((i64)d * B + b) * T + t;
+        dh[j] = 0.0f;
+        if (step < 0) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) gate[j][g] = gates[m[j] * 4 * H + g * H + uc];
+        c[j] = cells[m[j] * H + uc];
+        c_before[j] = step ? cells[(m[j] + before - t) * H + uc] : c0 ? c0[at[j]] : 0.0f;
+        dct[j] = step < T - 1 ? dc[at[j]] : gcn ? gcn[at[j]] : 0.0f;
+        if (step == T - 1 && ghn) dh[j] = ghn[at[j]];
+        if (gy) dh[j] += gy[((b * T + t) * s.dirs + d) * H + uc];
+    }
+    f32x4 acc[1][S] = {};
+    if (step < T - 1) {
+        const float *a[S], *v[1];
+#pragma unroll
+        for (int j = 0; j < S; ++j) a[j] = dz + (((i64)d * B + (p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1)) * T + after) * 4 * H;
+        v[0] = w_hh_t + ((i64)d * H + (p.u0 + (lane & 15) < H ? p.u0 + (lane & 15) : H - 1)) * 4 * H;
+        step_product<S, 1, 4, WIDE>(4 * H, a, v, acc);
+    }
+    float sum[S][1];
+    step_join<S, 1>(acc, lds, sum);
     if (u >= H) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int b = b0 + (threadIdx.x >> 6) * 16 + (lane >> 4) * 4 + r;
-        if (b >= B) continue;
-        const i64 at = ((i64)d * B + b) * H + u;
-        float dh = acc[0][r];
+    for (int j = 0; j < S; ++j) {
+        if (p.b0 + j * 16 + row >= B) continue;
+        dh[j] += sum[j][0];
         if (step < 0) {
-            dh0[at] = dh;
+            dh0[at[j]] = dh[j];
             continue;
         }
-        if (step == T - 1 && ghn) dh += ghn[at];
-        if (gy) dh += gy[(((i64)b * T + t) * s.dirs + d) * H + u];
-        const i64 row = ((i64)d * T + t) * B + b;
-        const float *a = gates + row * 4 * H + u, i = a[0], f = a[H], g = a[2 * H], o = a[3 * H];
-        const float c = tanh_of(cells[row * H + u]);
-        const float c_before = step ? cells[(((i64)d * T + before) * B + b) * H + u] : c0 ? c0[at] : 0.0f;
-        float dct = step < T - 1 ? dc[at] : gcn ? gcn[at] : 0.0f;
-        dct += dh * o * (1.0f - c * c);
-        float* q = dz + row * 4 * H + u;
-        q[0] = dct * g * i * (1.0f - i);
-        q[H] = dct * c_before * f * (1.0f - f);
-        q[2 * H] = dct * i * (1.0f - g * g);
-        q[3 * H] = dh * c * o * (1.0f - o);
-        dc[at] = dct * f;
+        const float i = gate[j][0], f = gate[j][1], g = gate[j][2], o = gate[j][3], tc = tanh_of(c[j]);
+        const float dcell = dct[j] + dh[j] * o * (1.0f - tc * tc);
+        float* q = dz + m[j] * 4 * H + u;
+        q[0] = dcell * g * i * (1.0f - i);
+        q[H] = dcell * c_before[j] * f * (1.0f - f);
+        q[2 * H] = dcell * i * (1.0f - g * g);
+        q[3 * H] = dh[j] * tc * o * (1.0f - o);
+        dc[at[j]] = dcell * f;
     }
 }
 
@@ -425,31 +490,45 @@ __global__ __launch_bounds__(256) void lstm_step_back_kernel(Shape s, int step, 
 const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
     if (dirs != 1 && dirs != 2) return "one direction or two";
     if (B < 0 || T < 1 || I < 1 || H < 1) return "sizes must be positive (the batch may be empty)";
-    if (I > 65536 || H > 8192) return "at most 65,536 inputs and 8,192 units";
+    if (I > 16384 || H > 8192) return "at most 16,384 inputs and 8,192 units";
     if (B > (1 << 22) || T > (1 << 22) || B * T >= (1ll << 30)) return "at most 2^22 sequences, 2^22 steps and 2^30 of both";
+    if (B * T * (H > I ? H : I) >= (1ll << 37)) return "the layer's activations would not fit any device";
     return nullptr;
 }
-// 128 x 128 tiles where they fill the device, else 64 x 64
-bool big_tiles(i64 m, i64 n, i64 z) { return cdiv(m, 128) * cdiv(n, 128) * z >= 256; }
 bool aligned(const void* p) { return (size_t)p % 16 == 0; }
 
-struct Split { int tile, parts, per_part, bias_parts, bias_per; };
-Split split_of(i64 B, i64 T, i64 I, i64 H, int dirs) {   // the sum over m of the weights' gradients, in parts
+// tiles of 128 x 128 where they fill the device twice, else of 64 x 64
+int tile_for(i64 m, i64 n) { return cdiv(m, 128) * cdiv(n, 128) >= 512 ? 128 : 64; }
+#define DSP_TILES(kernel, tile, fast, blocks, s, ...)                                                                                   \
+    do {                                                                                                                                \
+        if (tile == 128 && fast) hipLaunchKernelGGL((kernel<128, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);       \
+        else if (tile == 128) hipLaunchKernelGGL((kernel<128, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);         \
+        else if (fast) hipLaunchKernelGGL((kernel<64, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                  \
+        else hipLaunchKernelGGL((kernel<64, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                           \
+    } while (0)
+
+// 16-sequence blocks of a step's workgroup: as many (up to 4) as leave 256 workgroups
+int step_blocks(const Shape& s) {
+    for (int S = 4; S > 1; S >>= 1)
+        if (cdiv(s.B, 16 * S) * cdiv(s.H, 16) * s.dirs >= 256) return S;
+    return 1;
+}
+
+struct Split { int tile, parts, per_part; };
+// the sum over m of the weights' gradients, in parts: about 768 workgroups (3 a CU), and sums of no more than 4,096 products in a row
+Split split_of(i64 B, i64 T, i64 I, i64 H, int dirs) {
     Split q;
     const i64 M = 4 * H, K = B * T;
     q.tile = cdiv(M, 128) * (cdiv(I, 128) + cdiv(H, 128)) * dirs * cdiv(K, 512) >= 256 ? 128 : 64;
     const i64 tiles = cdiv(M, q.tile) * (cdiv(I, q.tile) + cdiv(H, q.tile)) * dirs;
-    i64 parts = cdiv(512, tiles);   // about two workgroups a CU
+    i64 parts = cdiv(768, tiles);
     if (parts > cdiv(K, 256)) parts = cdiv(K, 256);
+    if (parts < cdiv(K, 4096)) parts = cdiv(K, 4096);
     if (parts < 1) parts = 1;
     q.per_part = (int)(cdiv(cdiv(K, parts), kStep) * kStep);
     if (q.per_part < kStep) q.per_part = kStep;
     q.parts = (int)cdiv(K, q.per_part);
     if (q.parts < 1) q.parts = 1;
-    const i64 bias = cdiv(K, 256) < 64 ? cdiv(K, 256) : 64;
-    q.bias_per = (int)cdiv(K, bias < 1 ? 1 : bias);
-    if (q.bias_per < 1) q.bias_per = 1;
-    q.bias_parts = (int)cdiv(K, q.bias_per);
     return q;
 }
 
@@ -462,26 +541,40 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     const char* who = "dsp_lstm_forward";
     if (!l) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
-    if (l->batch == 0) return DSP_OK;
-    if (!x || !y || !hn || !cn || !gates || !cells) return refuse(who, "NULL pointer");
     Weights w = {};
-    bool wide_h = l->hidden % 4 == 0 && aligned(y) && aligned(h0), wide_wx = l->input % 4 == 0;
+    bool hidden_wide = l->hidden % 16 == 0 && aligned(y) && aligned(h0), input_wide = l->input % 16 == 0 && aligned(x);
     for (int d = 0; d < l->directions; ++d) {
         w.w_ih[d] = l->w_ih[d]; w.w_hh[d] = l->w_hh[d]; w.b_ih[d] = l->b_ih[d]; w.b_hh[d] = l->b_hh[d];
         if (!w.w_ih[d] || !w.w_hh[d] || !w.b_ih[d] || !w.b_hh[d]) return refuse(who, "NULL weight");
-        wide_h = wide_h && aligned(w.w_hh[d]);
-        wide_wx = wide_wx && aligned(w.w_ih[d]);
+        hidden_wide = hidden_wide && aligned(w.w_hh[d]);
+        input_wide = input_wide && aligned(w.w_ih[d]);
     }
-    const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, l->directions, l->input % 4 == 0 && aligned(x), wide_h, wide_wx};
+    if (l->batch == 0) return DSP_OK;
+    const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, l->directions};
+    const bool fused = s.T == 1;   // a single step makes the gates of x itself: nothing is gained by a product of its own
+    if (!x || !y || !hn || !cn || !cells || (!gates && (!fused || save))) return refuse(who, "NULL pointer");
     hipStream_t q = (hipStream_t)stream;
-    const i64 M = l->batch * l->steps, N = 4ll * s.H;
-    if (big_tiles(M, N, s.dirs))
-        hipLaunchKernelGGL(lstm_inputs_kernel<128>, dim3((unsigned)cdiv(M, 128), (unsigned)cdiv(N, 128), s.dirs), dim3(256), 0, q, s, x, w, gates);
-    else
-        hipLaunchKernelGGL(lstm_inputs_kernel<64>, dim3((unsigned)cdiv(M, 64), (unsigned)cdiv(N, 64), s.dirs), dim3(256), 0, q, s, x, w, gates);
-    const dim3 grid((unsigned)cdiv(s.B, kSeqs), (unsigned)cdiv(s.H, kUnits), s.dirs);
-    for (int step = 0; step < s.T; ++step)
-        hipLaunchKernelGGL(lstm_step_kernel, grid, dim3(256), 0, q, s, step, w, h0, c0, gates, cells, y, hn, cn, save);
+    const i64 M = l->batch * l->steps, N = 4ll * s.H, all = s.dirs * M * s.H;
+    if (!fused) {
+        const int tile = tile_for(M, N * s.dirs);
+        DSP_TILES(lstm_inputs_kernel, tile, input_wide, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
+    }
+    const int S = step_blocks(s);
+    const bool wide = hidden_wide && (!fused || input_wide);
+    const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * s.dirs));
+    for (int step = 0; step < s.T; ++step) {
+#define DSP_STEP(S, W, F) hipLaunchKernelGGL((lstm_step_kernel<S, W, F>), grid, dim3(256), 0, q, s, step, w, x, h0, c0, gates, cells, cells + all, y, hn, cn, save)
+#define DSP_STEP_OF(S)                                                                                       \
+    do {                                                                                                     \
+        if (fused) { if (wide) DSP_STEP(S, true, true); else DSP_STEP(S, false, true); }                     \
+        else { if (wide) DSP_STEP(S, true, false); else DSP_STEP(S, false, false); }                         \
+    } while (0)
+        if (S == 4) DSP_STEP_OF(4);
+        else if (S == 2) DSP_STEP_OF(2);
+        else DSP_STEP_OF(1);
+#undef DSP_STEP_OF
+#undef DSP_STEP
+    }
     return launched(who);
 }
 
@@ -490,71 +583,65 @@ int64_t dsp_lstm_workspace(const dsp_lstm_layer* l) {
     if (!l) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
     const Split p = split_of(l->batch, l->steps, l->input, l->hidden, l->directions);
-    size_t bytes = align256((size_t)l->directions * l->hidden * 4 * l->hidden * 4);                                     // W_hh transposed
-    bytes += align256((size_t)l->directions * l->steps * l->batch * 4 * l->hidden * 4);                                 // dz
-    if (p.parts > 1) bytes += align256((size_t)p.parts * l->directions * 4 * l->hidden * (l->input + l->hidden) * 4);   // parts of dW
-    return (int64_t)(bytes + align256((size_t)p.bias_parts * l->directions * 4 * l->hidden * 4));                       // parts of db
+    size_t bytes = align256((size_t)l->directions * l->hidden * 4 * l->hidden * 4);                                    // W_hh transposed
+    bytes += align256((size_t)l->directions * l->steps * l->batch * 4 * l->hidden * 4);                                // dz
+    return (int64_t)(bytes + align256((size_t)p.parts * l->directions * 4 * l->hidden * (l->input + l->hidden + 1) * 4));   // parts of dW and db
 }
 
-int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x, const float* h0, const float* c0, const float* y, const float* gates,
-                          const float* cells, const float* gy, const float* ghn, const float* gcn, float* dx, float* dh0, float* dc0,
-                          const dsp_lstm_grads* g, void* workspace, int64_t workspace_bytes) {
+int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x, const float* c0, const float* gates, const float* cells, const float* gy,
+                          const float* ghn, const float* gcn, float* dx, float* dh0, float* dc0, const dsp_lstm_grads* g, void* workspace,
+                          int64_t workspace_bytes) {
     const char* who = "dsp_lstm_backward";
     if (!l || !g) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
     const int dirs = l->directions;
-    for (int d = 0; d < dirs; ++d)
-        if (!l->w_ih[d] || !l->w_hh[d] || !g->w_ih[d] || !g->w_hh[d] || !g->b_ih[d] || !g->b_hh[d]) return refuse(who, "NULL weight or gradient");
-    if (l->batch && (!x || !y || !gates || !cells || !dc0 || !workspace)) return refuse(who, "NULL pointer");
-    if (workspace_bytes < dsp_lstm_workspace(l)) return refuse(who, "workspace too small (dsp_lstm_workspace)");
-    if (!workspace || ((size_t)workspace & 255)) return refuse(who, "the workspace must be aligned to 256 bytes");
     Weights w = {};
-    bool wide_wx = l->input % 4 == 0;
+    Grads out = {};
+    bool input_wide = l->input % 4 == 0 && aligned(x);
     for (int d = 0; d < dirs; ++d) {
         w.w_ih[d] = l->w_ih[d];
         w.w_hh[d] = l->w_hh[d];
-        wide_wx = wide_wx && aligned(w.w_ih[d]);
+        out.w_ih[d] = g->w_ih[d]; out.w_hh[d] = g->w_hh[d]; out.b_ih[d] = g->b_ih[d]; out.b_hh[d] = g->b_hh[d];
+        if (!w.w_ih[d] || !w.w_hh[d] || !out.w_ih[d] || !out.w_hh[d] || !out.b_ih[d] || !out.b_hh[d]) return refuse(who, "NULL weight or gradient");
+        input_wide = input_wide && aligned(w.w_ih[d]);
     }
-    const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, dirs, l->input % 4 == 0 && aligned(x),
-                     l->hidden % 4 == 0 && aligned(y) && aligned(h0), wide_wx};
+    if (l->batch && (!x || !gates || !cells || !dc0)) return refuse(who, "NULL pointer");
+    if (!workspace || workspace_bytes < dsp_lstm_workspace(l)) return refuse(who, "workspace too small (dsp_lstm_workspace)");
+    if ((size_t)workspace & 255) return refuse(who, "the workspace must be aligned to 256 bytes");
+    const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, dirs};
+    const i64 M = (i64)s.B * s.T;
+    const float* h_before = cells + dirs * M * s.H;
+    const bool hidden_wide = s.H % 4 == 0 && aligned(cells);
     const Split p = split_of(l->batch, l->steps, l->input, l->hidden, dirs);
     char* ws = (char*)workspace;
     float* wt = (float*)ws;
     ws += align256((size_t)dirs * s.H * 4 * s.H * 4);
     float* dz = (float*)ws;
     ws += align256((size_t)dirs * s.T * s.B * 4 * s.H * 4);
-    float* dw_part = (float*)ws;
-    if (p.parts > 1) ws += align256((size_t)p.parts * dirs * 4 * s.H * (s.I + s.H) * 4);
-    float* db_part = (float*)ws;
+    float* part = (float*)ws;
     hipStream_t q = (hipStream_t)stream;
-    const i64 M = (i64)s.B * s.T;
     if (s.B) {
         hipLaunchKernelGGL(lstm_transpose_kernel, dim3((unsigned)cdiv(s.H, 32), (unsigned)cdiv(4 * s.H, 32), dirs), dim3(256), 0, q, s.H, w, wt);
-        const dim3 grid((unsigned)cdiv(s.B, kSeqs), (unsigned)cdiv(s.H, kUnits), dirs);
-        for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step)
-            hipLaunchKernelGGL(lstm_step_back_kernel, grid, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0);
+        const int S = step_blocks(s);
+        const bool wide = s.H % 4 == 0;   // 4H in steps of 16, from the workspace
+        const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * dirs));
+        for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step) {
+#define DSP_BACK(S, W) hipLaunchKernelGGL((lstm_step_back_kernel<S, W>), grid, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0)
+            if (S == 4) { if (wide) DSP_BACK(4, true); else DSP_BACK(4, false); }
+            else if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
+            else { if (wide) DSP_BACK(1, true); else DSP_BACK(1, false); }
+#undef DSP_BACK
+        }
         if (dx) {
-            if (big_tiles(M, s.I, 1))
-                hipLaunchKernelGGL(lstm_input_grad_kernel<128>, dim3((unsigned)cdiv(M, 128), (unsigned)cdiv(s.I, 128)), dim3(256), 0, q, s, (const float*)dz, w, dx);
-            else
-                hipLaunchKernelGGL(lstm_input_grad_kernel<64>, dim3((unsigned)cdiv(M, 64), (unsigned)cdiv(s.I, 64)), dim3(256), 0, q, s, (const float*)dz, w, dx);
+            const int tile = tile_for(M, s.I);
+            const bool fast = input_wide && s.H % 4 == 0;
+            DSP_TILES(lstm_input_grad_kernel, tile, fast, cdiv(M, tile) * cdiv(s.I, tile), q, s, (const float*)dz, w, dx);
         }
     }
-    const int x_tiles = (int)cdiv(s.I, p.tile);
-    const dim3 grid((unsigned)(x_tiles + cdiv(s.H, p.tile)), (unsigned)cdiv(4 * s.H, p.tile), (unsigned)(dirs * p.parts));
-    if (p.tile == 128)
-        hipLaunchKernelGGL(lstm_weight_grad_kernel<128>, grid, dim3(256), 0, q, s, (const float*)dz, x, y, h0, p.parts, p.per_part, x_tiles, dw_part, g->w_ih[0],
-                           g->w_ih[1], g->w_hh[0], g->w_hh[1]);
-    else
-        hipLaunchKernelGGL(lstm_weight_grad_kernel<64>, grid, dim3(256), 0, q, s, (const float*)dz, x, y, h0, p.parts, p.per_part, x_tiles, dw_part, g->w_ih[0],
-                           g->w_ih[1], g->w_hh[0], g->w_hh[1]);
-    if (p.parts > 1)
-        hipLaunchKernelGGL(lstm_join_kernel, dim3((unsigned)cdiv((i64)dirs * 4 * s.H * (s.I + s.H), 256)), dim3(256), 0, q, s, p.parts, (const float*)dw_part,
-                           g->w_ih[0], g->w_ih[1], g->w_hh[0], g->w_hh[1]);
-    if (p.bias_parts)
-        hipLaunchKernelGGL(lstm_bias_grad_kernel, dim3((unsigned)cdiv(4 * s.H, 64), (unsigned)p.bias_parts, dirs), dim3(256), 0, q, s, (const float*)dz, p.bias_per, db_part);
-    hipLaunchKernelGGL(lstm_bias_join_kernel, dim3((unsigned)cdiv(4 * s.H * dirs, 256)), dim3(256), 0, q, s, p.bias_parts, (const float*)db_part, g->b_ih[0], g->b_ih[1],
-                       g->b_hh[0], g->b_hh[1]);
+    const bool fast = input_wide && hidden_wide && (i64)p.per_part * 4 * (s.I > 4 * s.H ? s.I : 4 * s.H) < (1ll << 31);
+    DSP_TILES(lstm_weight_grad_kernel, p.tile, fast, cdiv(4 * s.H, p.tile) * (cdiv(s.I, p.tile) + cdiv(s.H, p.tile)) * dirs * p.parts, q, s, (const float*)dz, x,
+              h_before, p.per_part, part);
+    hipLaunchKernelGGL(lstm_join_kernel, dim3((unsigned)cdiv((i64)dirs * 4 * s.H * (s.I + s.H + 1), 256)), dim3(256), 0, q, s, p.parts, (const float*)part, out);
     return launched(who);
 }
 

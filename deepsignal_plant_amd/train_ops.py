@@ -18,6 +18,7 @@ import math
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 
@@ -28,44 +29,62 @@ _REDUCE = {"mean": 0, "sum": 1, "none": 2}
 
 
 def _one_gpu(who, *tensors):
-    """the tensors' GPU (None among them: not given)"""
-    dev = None
+    """the index of the tensors' GPU (None among them: not given)"""
+    dev = -1
     for t in tensors:
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s: expected a tensor, got %s" % (who, type(t).__name__))
-        if not t.is_cuda:
-            raise RuntimeError("%s: tensors must live on a GPU (no CPU path)" % who)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError("%s: tensors on %s and %s" % (who, dev, t.device))
+        at = t.get_device()
+        if at != dev or dev < 0:
+            if at < 0:
+                raise RuntimeError("%s: tensors must live on a GPU (no CPU path)" % who)
+            if dev >= 0:
+                raise RuntimeError("%s: tensors on cuda:%d and cuda:%d" % (who, dev, at))
+            dev = at
     return dev
 
 
+# the stream handle alone; the Stream object that the public call makes costs 2 us of a call of 10
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _call(dev, fn, *args):
-    """one call of the library on `dev` and its current stream"""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        return nat.check(fn(stream, *args))
-    with torch.cuda.device(dev):
-        return nat.check(fn(stream, *args))
+    """one call of the library on GPU `dev` and its current stream"""
+    if torch.cuda.current_device() == dev:
+        rc = fn(_raw_stream(dev), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(_raw_stream(dev), *args)
+    if rc:
+        nat.check(rc)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(dev, size):
-    return torch.empty(nat.check(size), dtype=torch.uint8, device=dev)
+def _workspace(like, size):
+    return like.new_empty(nat.check(size), dtype=torch.uint8)
+
+
+def _differentiable_once(backward):
+    """autograd.function.once_differentiable, whose wrapping is skipped where no graph of the backward pass is asked for (it costs
+    several microseconds)"""
+    with_graph = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return with_graph(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(run)
 
 
 # ---- embedding ----------------------------------------------------------------------------------------------------------------
 def _embedding_forward(tokens, weight, scale):
-    out = torch.empty(tokens.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
-    _call(weight.device, nat.lib().dsp_embedding_forward, tokens.numel(), tokens.data_ptr(), _TOKEN[tokens.dtype], weight.data_ptr(), weight.shape[0],
-          weight.shape[1], _FLOAT[weight.dtype], scale, out.data_ptr())
+    rows, dim = weight.shape
+    out = weight.new_empty((*tokens.shape, dim))
+    _call(weight.get_device(), nat.lib().dsp_embedding_forward, tokens.numel(), tokens.data_ptr(), _TOKEN[tokens.dtype], weight.data_ptr(), rows, dim,
+          _FLOAT[weight.dtype], scale, out.data_ptr())
     return out
 
 
@@ -73,19 +92,19 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding_idx):
         ctx.save_for_backward(tokens)
-        ctx.table, ctx.scale, ctx.padding_idx = weight.shape, scale, padding_idx
+        ctx.how = *weight.shape, scale, padding_idx
         return _embedding_forward(tokens, weight, scale)
 
-    @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, grad):
         tokens, = ctx.saved_tensors
-        (vocab, dim), n, L = ctx.table, tokens.numel(), nat.lib()
+        rows, dim, scale, padding_idx = ctx.how
+        n, L = tokens.numel(), nat.lib()
         grad = grad.contiguous()
-        out = torch.empty(ctx.table, dtype=grad.dtype, device=grad.device)
-        ws = _workspace(grad.device, L.dsp_embedding_workspace(n, vocab, dim))
-        _call(grad.device, L.dsp_embedding_backward, n, tokens.data_ptr(), _TOKEN[tokens.dtype], grad.data_ptr(), vocab, dim, _FLOAT[grad.dtype],
-              ctx.padding_idx, ctx.scale, out.data_ptr(), ws.data_ptr(), ws.numel())
+        out = grad.new_empty((rows, dim))
+        ws = _workspace(grad, L.dsp_embedding_workspace(n, rows, dim))
+        _call(grad.get_device(), L.dsp_embedding_backward, n, tokens.data_ptr(), _TOKEN[tokens.dtype], grad.data_ptr(), rows, dim, _FLOAT[grad.dtype],
+              padding_idx, scale, out.data_ptr(), ws.data_ptr(), ws.numel())
         return None, out, None, None
 
 
@@ -103,16 +122,18 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError("embedding: scale must be finite")
-    pad = -1
+    pad = -1   # none
     if padding_idx is not None:
         pad = int(padding_idx)
         if not -weight.shape[0] <= pad < weight.shape[0]:
             raise ValueError("embedding: padding_idx %d is not a row of the table" % pad)
         pad %= weight.shape[0]
-    tokens = tokens.detach().contiguous()
+    tokens = tokens.contiguous()
+    if tokens.requires_grad:
+        tokens = tokens.detach()
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(tokens, weight.contiguous(), scale, pad)
-    return _embedding_forward(tokens, weight.detach().contiguous(), scale)
+    return _embedding_forward(tokens, weight.contiguous(), scale)
 
 
 # ---- lstm -----------------------------------------------------------------------------------------------------------------------
@@ -125,11 +146,11 @@ def _layer(x, weights):
 
 
 def _lstm_forward(x, h0, c0, weights, save):
-    l, dev = _layer(x, weights), x.device
+    l, new = _layer(x, weights), x.new_empty
     B, T, H, D = l.batch, l.steps, l.hidden, l.directions
-    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
-    y, hn, cn, gates, cells = new(B, T, D * H), new(D, B, H), new(D, B, H), new(D, T, B, 4 * H), new(D, T if save else 2, B, H)
-    _call(dev, nat.lib().dsp_lstm_forward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), hn.data_ptr(), cn.data_ptr(), gates.data_ptr(),
+    y, hn, cn, cells = new((B, T, D * H)), new((D, B, H)), new((D, B, H)), new((2, D, B, T if save else 1, H))
+    gates = new((D, B, T, 4 * H)) if save or T > 1 else None
+    _call(x.get_device(), nat.lib().dsp_lstm_forward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), hn.data_ptr(), cn.data_ptr(), _ptr(gates),
           cells.data_ptr(), int(save))
     return y, hn, cn, gates, cells
 
@@ -138,27 +159,26 @@ class _Lstm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h0, c0, *weights):
         y, hn, cn, gates, cells = _lstm_forward(x, h0, c0, weights, True)
-        ctx.save_for_backward(x, h0, c0, y, gates, cells, *weights)
+        ctx.save_for_backward(x, c0, gates, cells, *weights)
         ctx.set_materialize_grads(False)
         return y, hn, cn
 
-    @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, gy, ghn, gcn):
-        x, h0, c0, y, gates, cells, *weights = ctx.saved_tensors
-        l, dev, L = _layer(x, weights), x.device, nat.lib()
+        x, c0, gates, cells, *weights = ctx.saved_tensors
+        l, L = _layer(x, weights), nat.lib()
         gy, ghn, gcn = (None if g is None else g.contiguous() for g in (gy, ghn, gcn))
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         states = (l.directions, l.batch, l.hidden)
-        dh0 = torch.empty(states, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-        dc0 = torch.empty(states, dtype=torch.float32, device=dev)
+        dh0 = x.new_empty(states) if ctx.needs_input_grad[1] else None
+        dc0 = x.new_empty(states)
         dws = [torch.empty_like(w) for w in weights]
         g = nat.LstmGrads()
         for d in range(l.directions):
             g.w_ih[d], g.w_hh[d], g.b_ih[d], g.b_hh[d] = (w.data_ptr() for w in dws[4 * d:4 * d + 4])
-        ws = _workspace(dev, L.dsp_lstm_workspace(ctypes.byref(l)))
-        _call(dev, L.dsp_lstm_backward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), gates.data_ptr(), cells.data_ptr(), _ptr(gy),
-              _ptr(ghn), _ptr(gcn), _ptr(dx), _ptr(dh0), dc0.data_ptr(), ctypes.byref(g), ws.data_ptr(), ws.numel())
+        ws = _workspace(x, L.dsp_lstm_workspace(ctypes.byref(l)))
+        _call(x.get_device(), L.dsp_lstm_backward, ctypes.byref(l), x.data_ptr(), _ptr(c0), gates.data_ptr(), cells.data_ptr(), _ptr(gy), _ptr(ghn),
+              _ptr(gcn), _ptr(dx), _ptr(dh0), dc0.data_ptr(), ctypes.byref(g), ws.data_ptr(), ws.numel())
         return (dx, dh0, dc0 if ctx.needs_input_grad[2] else None, *dws)
 
 
@@ -169,7 +189,7 @@ def lstm(x, weights, h0=None, c0=None):
     weights: weight_ih [4 * hidden, input], weight_hh [4 * hidden, hidden], bias_ih, bias_hh [4 * hidden], and the same four of the
     reverse direction for a bidirectional layer (the order of the state_dict; gates i, f, g, o).  h0, c0 [directions, batch,
     hidden]: zeros where not given.  One step with the states handed on is the form for running sequences.  The gradient costs
-    memory of 9 * hidden values a step, sequence and direction from the forward to the backward pass; under torch.no_grad none."""
+    memory of 6 * hidden values a step, sequence and direction from the forward to the backward pass; under torch.no_grad none."""
     weights = list(weights)
     if len(weights) not in (4, 8):
         raise ValueError("lstm: expected the 4 weights of one direction or the 8 of two, got %d" % len(weights))
@@ -201,37 +221,36 @@ def _loss_args(logits, labels, weight, ignore_index, reduction):
 
 
 def _loss_forward(logits, labels, weight, ignore_index, reduction, want_grad):
-    dev, n, L = logits.device, logits.shape[0], nat.lib()
-    loss = torch.empty((n,) if reduction == 2 else (), dtype=torch.float32, device=dev)
-    stat = torch.empty((n, 2), dtype=torch.float32, device=dev)
-    total = torch.empty((), dtype=torch.float64, device=dev)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad and reduction != 2 else None
-    ws = _workspace(dev, L.dsp_cross_entropy_workspace(n))
-    _call(dev, L.dsp_cross_entropy_forward, *_loss_args(logits, labels, weight, ignore_index, reduction), loss.data_ptr(), stat.data_ptr(), total.data_ptr(),
+    n, L = logits.shape[0], nat.lib()
+    loss = logits.new_empty((n,) if reduction == 2 else (), dtype=torch.float32)
+    keep = logits.new_empty(1 + n, dtype=torch.float64)   # the sum of the weights, and two float32 of each row
+    grad = logits.new_empty(logits.shape) if want_grad and reduction != 2 else None
+    ws = _workspace(logits, L.dsp_cross_entropy_workspace(n))
+    at = keep.data_ptr()
+    _call(logits.get_device(), L.dsp_cross_entropy_forward, *_loss_args(logits, labels, weight, ignore_index, reduction), loss.data_ptr(), at + 8, at,
           _ptr(grad), ws.data_ptr(), ws.numel())
-    return loss, stat, total, grad
+    return loss, keep, grad
 
 
 class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, weight, ignore_index, reduction):
-        loss, stat, total, ctx.unit_grad = _loss_forward(logits, labels, weight, ignore_index, reduction, True)
-        ctx.save_for_backward(logits, labels, weight, stat, total)
+        loss, keep, ctx.unit_grad = _loss_forward(logits, labels, weight, ignore_index, reduction, True)
+        ctx.save_for_backward(logits, labels, weight, keep)
         ctx.how = ignore_index, reduction
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, upstream):
-        logits, labels, weight, stat, total = ctx.saved_tensors
+        logits, labels, weight, keep = ctx.saved_tensors
         # the gradient that the forward pass left is handed out once; a second pass over a retained graph computes its own
         grad, ctx.unit_grad = ctx.unit_grad, None
         unit = grad is not None
         if not unit:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        upstream = upstream.contiguous()
-        _call(logits.device, nat.lib().dsp_cross_entropy_backward, *_loss_args(logits, labels, weight, *ctx.how), stat.data_ptr(), total.data_ptr(),
-              upstream.data_ptr(), int(unit), grad.data_ptr())
+            grad = logits.new_empty(logits.shape)
+        upstream, at = upstream.contiguous(), keep.data_ptr()
+        _call(logits.get_device(), nat.lib().dsp_cross_entropy_backward, *_loss_args(logits, labels, weight, *ctx.how), at + 8, at, upstream.data_ptr(), int(unit),
+              grad.data_ptr())
         return grad, None, None, None, None
 
 
@@ -277,35 +296,49 @@ def _is_dense(t):
 
 
 def _check_grads(who, grads):
+    """the index of their GPU"""
     for g in grads:
-        if not isinstance(g, torch.Tensor) or g.layout != torch.strided:
+        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided:
             raise ValueError("%s: gradients must be dense tensors" % who)
         if g.dtype not in _FLOAT:
             raise ValueError("%s: gradients must be float32, bfloat16 or float16, got %s" % (who, g.dtype))
     return _one_gpu(who, *grads)
 
 
-def _spans(tensors):
-    return [(p, p + t.numel() * t.element_size()) for t in tensors for p in (t.data_ptr(),) if t.numel()]
+class _Pieces(object):
+    """where tensors lie: addresses, numbers of values, types, and (start, end) of those that are not empty in order"""
+
+    def __init__(self, tensors):
+        self.ptrs = [t.data_ptr() for t in tensors]
+        self.numels = [t.numel() for t in tensors]
+        self.types = [_FLOAT[t.dtype] for t in tensors]
+        self.spans = sorted([(p, p + n * (2 if t else 4)) for p, n, t in zip(self.ptrs, self.numels, self.types) if n])
+
+    def check_apart(self, who):
+        end = 0
+        for start, stop in self.spans:
+            if start < end:
+                raise ValueError("%s: tensors that are written overlap in memory" % who)
+            end = stop
+
+    def check_apart_from(self, who, others):
+        other = iter(others.spans)
+        at = next(other, None)
+        for start, end in self.spans:
+            while at and at[1] <= start:
+                at = next(other, None)
+            if at and at[0] < end:
+                raise ValueError("%s: an output overlaps a gradient (clip_grad_norm_ works in place)" % who)
 
 
-def _check_apart(who, spans):
-    spans.sort()
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise ValueError("%s: tensors that are written overlap in memory" % who)
-
-
-def _run_clip(dev, grads, outs, max_norm):
-    n = len(grads)
-    ptr, i64, i32 = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int32 * n
-    numels = i64(*[g.numel() for g in grads])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    L = nat.lib()
-    ws = _workspace(dev, L.dsp_clip_workspace(n, numels))
-    _call(dev, L.dsp_clip_grad_norm, n, ptr(*[g.data_ptr() for g in grads]), numels, i32(*[_FLOAT[g.dtype] for g in grads]),
-          None if outs is None else ptr(*[o.data_ptr() for o in outs]), None if outs is None else i32(*[_FLOAT[o.dtype] for o in outs]), max_norm,
-          norm.data_ptr(), ws.data_ptr(), ws.numel())
+def _run_clip(dev, like, grads, outs, max_norm):
+    n, L = len(grads.ptrs), nat.lib()
+    ptr, i32 = ctypes.c_void_p * n, ctypes.c_int32 * n
+    numels = (ctypes.c_int64 * n)(*grads.numels)
+    norm = like.new_empty((), dtype=torch.float32)
+    ws = _workspace(like, L.dsp_clip_workspace(n, numels))
+    _call(dev, L.dsp_clip_grad_norm, n, ptr(*grads.ptrs), numels, i32(*grads.types), None if outs is None else ptr(*outs.ptrs),
+          None if outs is None else i32(*outs.types), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
     return norm
 
 
@@ -320,10 +353,11 @@ def _max_norm(who, max_norm):
 def grad_norm(grads):
     """The 2-norm over all values of a list of tensors, as a float32 scalar on their GPU; squares and sums are held in 64 bits."""
     grads = list(grads)
-    dev = _check_grads("grad_norm", grads)
-    if dev is None:
+    if not grads:
         raise ValueError("grad_norm: no tensors")
-    return _run_clip(dev, [g if _is_dense(g) else g.contiguous() for g in grads], None, 0.0)
+    dev = _check_grads("grad_norm", grads)
+    grads = [g if _is_dense(g) else g.contiguous() for g in grads]
+    return _run_clip(dev, grads[0], _Pieces(grads), None, 0.0)
 
 
 @torch.no_grad()
@@ -334,26 +368,23 @@ def clip_grad_norm(grads, max_norm, out=None):
     32-bit weights takes); new ones where it is not given.  The gradients are left as they are."""
     who, grads = "clip_grad_norm", list(grads)
     max_norm = _max_norm(who, max_norm)
-    dev = _check_grads(who, grads)
-    if dev is None:
+    if not grads:
         raise ValueError("clip_grad_norm: no tensors")
-    out = [torch.empty(g.shape, dtype=g.dtype, device=dev) for g in grads] if out is None else list(out)
+    dev = _check_grads(who, grads)
+    out = [g.new_empty(g.shape) for g in grads] if out is None else list(out)
     if len(out) != len(grads):
         raise ValueError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
     _one_gpu(who, grads[0], *out)
     for g, o in zip(grads, out):
-        if o.shape != g.shape or not o.is_contiguous() or (o.dtype != g.dtype and o.dtype != torch.float32):
+        if o.shape != g.shape or not o.is_contiguous() or (o.dtype is not g.dtype and o.dtype is not torch.float32):
             raise ValueError("clip_grad_norm: an output must be contiguous, of its gradient's shape, and of its type or float32")
     grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    outs = _spans(out)
-    _check_apart(who, outs)
-    ins, i = sorted(_spans(grads)), 0
-    for start, end in outs:   # both in order of their addresses, the outputs apart from each other
-        while i < len(ins) and ins[i][1] <= start:
-            i += 1
-        if i < len(ins) and ins[i][0] < end:
-            raise ValueError("clip_grad_norm: an output overlaps a gradient (clip_grad_norm_ works in place)")
-    return _run_clip(dev, grads, out, max_norm), out
+    ins, outs = _Pieces(grads), _Pieces(out)
+    outs.check_apart(who)
+    outs.check_apart_from(who, ins)
+    norm = _run_clip(dev, grads[0], ins, outs, max_norm)
+    increment_version(out)   # as torch's own writes do: a graph that saved one of them notices
+    return norm, out
 
 
 @torch.no_grad()
@@ -377,12 +408,14 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     for g, u in zip(grads, use):
         if u is not g and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
             raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
-    _check_apart(who, _spans(use))
+    pieces = _Pieces(use)
+    pieces.check_apart(who)
     if error_if_nonfinite:
-        norm = _run_clip(dev, use, None, 0.0)
+        norm = _run_clip(dev, use[0], pieces, None, 0.0)
         if not math.isfinite(norm.item()):
             raise RuntimeError("clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped")
-    norm = _run_clip(dev, use, use, max_norm)
+    norm = _run_clip(dev, use[0], pieces, pieces, max_norm)
+    increment_version(use)
     for g, u in zip(grads, use):
         if u is not g:
             g.copy_(u)

@@ -583,16 +583,23 @@ def test_lstm_saturated_gates_and_large_inputs(ops):
 
 
 def test_lstm_a_sequence_in_pieces_is_the_sequence(ops):
-    """the states of one call handed to the next, down to single steps: the same bits as one call"""
+    """the states of one call handed to the next: the same bits as one call for pieces of two steps and more.  A single step adds
+    W_ih x to the other products in an order of its own: each order is off by at most check_lstm's bound, both by twice that"""
     x, ws, h0, c0, _ = lstm_case(18, 9, 12, 36, dirs=1)
-    x, ws, h, c = x.to(DEV), [w.to(DEV) for w in ws], h0.to(DEV), c0.to(DEV)
-    with torch.no_grad():
-        y, hn, cn = ops.lstm(x, ws, h, c)
-        got = []
-        for a, b in ((0, 4), (4, 5), (5, 6), (6, 9)):
+    x, ws, h0, c0 = x.to(DEV), [w.to(DEV) for w in ws], h0.to(DEV), c0.to(DEV)
+
+    def pieces(*cuts):
+        got, h, c = [], h0, c0
+        for a, b in zip((0,) + cuts, cuts + (9,)):
             o, h, c = ops.lstm(x[:, a:b], ws, h, c)
             got.append(o)
-    assert torch.equal(torch.cat(got, 1), y) and torch.equal(h, hn) and torch.equal(c, cn)
+        return torch.cat(got, 1), h, c
+    with torch.no_grad():
+        whole = ops.lstm(x, ws, h0, c0)
+        assert all(torch.equal(a, b) for a, b in zip(pieces(4, 6), whole))
+        for cuts in ((4, 5, 6), tuple(range(1, 9))):
+            for got, want in zip(pieces(*cuts), whole):
+                near(got, want.double().cpu(), 2 * (4 * 36 + 12 + 40) * 10 * U, "pieces")
 
 
 def test_lstm_not_finite_stays_in_its_sequence(ops):

@@ -61,16 +61,17 @@ def test_lstm_refusals_at_the_abi():
     for bad in (dict(steps=0), dict(inputs=0), dict(hidden=0), dict(batch=-1)):
         refused(fwd(layer(**bad)), "positive")
     refused(fwd(layer(hidden=8193)), "8,192 units")
-    refused(fwd(layer(inputs=65537)), "65,536 inputs")
+    refused(fwd(layer(inputs=16385)), "16,384 inputs")
     refused(fwd(layer(batch=2 ** 22 + 1)), "2^22 sequences")
     refused(fwd(layer(batch=2 ** 15, steps=2 ** 15)), "2^30 of both")
     refused(fwd(layer(missing=("b_hh", 1))), "NULL weight")
+    refused(fwd(layer(batch=2 ** 20, steps=2 ** 9, hidden=2 ** 10)), "would not fit")
     refused(fwd(layer(), x=None), "NULL pointer")
     refused(fwd(layer(), y=None), "NULL pointer")
     assert fwd(layer(batch=0), x=None, y=None) == 0
     l = layer()
     size, g = L.dsp_lstm_workspace(ctypes.byref(l)), nat.LstmGrads()
-    bwd = lambda g, dc0=P, ws=P, size=size, l=l: L.dsp_lstm_backward(None, ctypes.byref(l), P, None, None, P, P, P, None, None, None, None, None, dc0,
+    bwd = lambda g, dc0=P, ws=P, size=size, l=l: L.dsp_lstm_backward(None, ctypes.byref(l), P, None, P, P, None, None, None, None, None, dc0,
                                                                   None if g is None else ctypes.byref(g), ws, size)
     refused(bwd(None), "NULL layer")
     refused(bwd(g), "NULL weight or gradient")
