@@ -179,7 +179,7 @@ struct Shape { int B, T, I, H, dirs; };
 struct Weights { const float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
 
 // gates = W_ih x + b_ih + b_hh, all steps
-template <int TILE, bool FAST> __global__ __launch_bounds__(256) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
+template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
     __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, TILE>()];
     const int M = s.B * s.T, N = 4 * s.H, n_tiles = (N + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
@@ -191,7 +191,7 @@ template <int TILE, bool FAST> __global__ __launch_bounds__(256) void lstm_input
 }
 
 // dx = sum over directions of dz W_ih
-template <int TILE, bool FAST> __global__ __launch_bounds__(256) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
+template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
     __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, false, TILE>()];
     const int M = s.B * s.T, K = 4 * s.H, n_tiles = (s.I + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
@@ -273,48 +273,83 @@ __device__ __forceinline__ float tanh_of(float x) {
 }
 
 // A workgroup of 4 waves makes a tile of 16 S sequences by C blocks of 16 columns (forward: the 4 gates of 16 units; backward: 16 units).
-// Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves: it goes from memory straight into
-// the registers in which v_mfma_f32_16x16x4 takes it (4 consecutive k a lane, as above), without LDS and barriers, D accesses ahead.
-// The quarters are joined through LDS at the end, in order.  WIDE: k comes in whole accesses of 4 and steps of 16.
-// a[i], w[i]: the lane's row of the i-th 16 rows.  Rows behind the last are clamped to it: what they give is not used.
-template <int S, int C, int D, bool WIDE> __device__ __forceinline__ void step_product(int K, const float* const (&a)[S], const float* const (&w)[C], f32x4 (&acc)[C][S]) {
-    const int q = (threadIdx.x & 63) >> 4, wave = threadIdx.x >> 6;
-    const int steps = (K + 15) >> 4, per = (steps + 3) >> 2, from = wave * per, to = from + per < steps ? from + per : steps;
-    f32x4 fa[D][S], fw[D][C];
-    auto load = [&](const float* p, int k) {
-        if (WIDE) return *(const f32x4*)(p + k);
-        f32x4 v;
+// Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves.  It loads lines of 128 bytes, 8 rows at a
+// time, 32 values of k ahead, and turns them in LDS of its own into what v_mfma_f32_16x16x4 takes (a lane's 4 consecutive k of one
+// row, as above).  Loaded in that form from memory they would cost the L1 an access for each 16 bytes: 16 neighbouring lanes are 16
+// rows (measured: 48 accesses a load, the L1 busy for 80 % of the time, 90 us a step of 4,096 sequences instead of 70).  No wave
+// waits for another until the quarters are joined, in order.  WIDE: rows begin at multiples of 16 bytes and k is one of 4.
+constexpr int kLine = 32;   // values of k at a time
+// where 4 values of a row lie in LDS: the 8 places of a row change with the pair of rows, so that 16 rows read at once fall on all banks
+__device__ __forceinline__ int spread(int row, int k) { return row * kLine + (((k >> 2) ^ (row >> 1)) & 7) * 4; }
+
+// row_a(i): the tile's i-th row;  col_w(i): the tile's i-th column as its offset in bytes from w, below 2^32
+template <int S, int C, bool WIDE, class RowA, class ColW>
+__device__ __forceinline__ void step_product(int K, RowA row_a, const float* w, ColW col_w, float* lds, f32x4 (&acc)[C][S]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = lane >> 3, on = (lane & 7) * 4;
+    const int lines = (K + kLine - 1) / kLine, per = (lines + 3) >> 2, from = wave * per, to = from + per < lines ? from + per : lines;
+    if (from >= to) return;
+    float *la = lds + wave * (S + C) * 16 * kLine, *lw = la + S * 16 * kLine;
+    const float* pa[2 * S];
+    uint32_t pw[2 * C];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < K ? p[k + e] : 0.0f;
-        return v;
+    for (int i = 0; i < 2 * S; ++i) pa[i] = row_a(i * 8 + at) + on;
+#pragma unroll
+    for (int i = 0; i < 2 * C; ++i) pw[i] = col_w(i * 8 + at) + on * 4;
+    f32x4 va[2 * S], vw[2 * C];
+    auto fetch = [&](int line) {
+        const int k = line * kLine;
+        const char* wk = (const char*)(w + k);
+        if (WIDE && k + kLine <= K) {
+#pragma unroll
+            for (int i = 0; i < 2 * S; ++i) va[i] = *(const f32x4*)(pa[i] + k);
+#pragma unroll
+            for (int i = 0; i < 2 * C; ++i) vw[i] = *(const f32x4*)(wk + pw[i]);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = k + on + e < K;
+#pragma unroll
+            for (int i = 0; i < 2 * S; ++i) va[i][e] = in ? pa[i][k + e] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * C; ++i) vw[i][e] = in ? *(const float*)(wk + pw[i] + e * 4) : 0.0f;
+        }
     };
-    auto fetch = [&](int i, int step) {
+    fetch(from);
+    for (int line = from; line < to; ++line) {
+        // one wave's accesses to LDS are carried out in order, and no other wave reads or writes here
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int j = 0; j < S; ++j) fa[i][j] = load(a[j], step * 16 + q * 4);
+        for (int i = 0; i < 2 * S; ++i) *(f32x4*)(la + spread(i * 8 + at, on)) = va[i];
 #pragma unroll
-        for (int j = 0; j < C; ++j) fw[i][j] = load(w[j], step * 16 + q * 4);
-    };
+        for (int i = 0; i < 2 * C; ++i) *(f32x4*)(lw + spread(i * 8 + at, on)) = vw[i];
+        __builtin_amdgcn_wave_barrier();
+        if (line + 1 < to) fetch(line + 1);
 #pragma unroll
-    for (int i = 0; i < D; ++i)
-        if (from + i < to) fetch(i, from + i);
-    for (int step = from; step < to; step += D)
+        for (int half = 0; half < 2; ++half) {
+            f32x4 fa[S], fw[C];
+            const int k = half * 16 + (lane >> 4) * 4;
 #pragma unroll
-        for (int i = 0; i < D; ++i) {
-            if (step + i >= to) break;
+            for (int j = 0; j < S; ++j) fa[j] = *(const f32x4*)(la + spread(j * 16 + (lane & 15), k));
+#pragma unroll
+            for (int c = 0; c < C; ++c) fw[c] = *(const f32x4*)(lw + spread(c * 16 + (lane & 15), k));
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < C; ++c)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i][j][e], fw[i][c][e], acc[c][j], 0, 0, 0);
-            if (step + i + D < to) fetch(i, step + i + D);
+                    for (int j = 0; j < S; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j][e], fw[c][e], acc[c][j], 0, 0, 0);
         }
+    }
 }
-// the sums of the 4 waves: f(c, row, unit, value) -- of every value of the tile, a thread's rows 16 apart
+// the sums of the 4 waves: of the values of the tile at the thread's rows (16 apart) and column
 constexpr int kRow = 17;   // floats of a row of 16 in LDS
-template <int S, int C> constexpr int step_floats() { return 4 * C * S * 16 * kRow; }
+template <int S, int C> constexpr int step_floats() {
+    return 4 * (S + C) * 16 * kLine > 4 * C * S * 16 * kRow ? 4 * (S + C) * 16 * kLine : 4 * C * S * 16 * kRow;
+}
 template <int S, int C> __device__ __forceinline__ void step_join(const f32x4 (&acc)[C][S], float* lds, float (&sum)[S][C]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();   // the waves are done with their parts of LDS
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -349,20 +384,20 @@ template <int S> __device__ __forceinline__ Place place_of(const Shape& s) {
 // gates: in W_ih x + b of all steps (FUSED: made here, from x); out (save) i, f, g, o.  cells: c of all steps (save), else of two steps
 // in turn; h_before (save): h before each step
 template <int S, bool WIDE, bool FUSED>
-__global__ __launch_bounds__(256) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ x, const float* __restrict__ h0,
+__global__ __launch_bounds__(256, 3) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ x, const float* __restrict__ h0,
                                                         const float* __restrict__ c0, float* gates, float* cells, float* h_before, float* y,
                                                         float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ float lds[step_floats<S, 4>()];
+    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 4>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15);
-    // what the gates need besides, on its way meanwhile
+    const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15);
+    // what the gates need besides the product, on its way meanwhile
     float z[S][4], c[S];
-    const int uc = u < H ? u : H - 1;
     i64 at[S], m[S];
+    const int uc = u < H ? u : H - 1;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-        const int b = p.b0 + j * 16 + row < B ? p.b0 + j * 16 + row : B - 1;
+        const i64 b = p.b0 + j * 16 + row < B ? p.b0 + j * 16 + row : B - 1;
         at[j] = ((i64)d * B + b) * H + uc;
         m[j] = ((i64)d * B + b) * T + t;
 #pragma unroll
@@ -372,25 +407,15 @@ __global__ __launch_bounds__(256) void lstm_step_kernel(Shape s, int step, Weigh
         else if (c0) c[j] = c0[at[j]];
     }
     f32x4 acc[4][S] = {};
-    const float *a[S], *v[4];
-    const int wu = p.u0 + (lane & 15) < H ? p.u0 + (lane & 15) : H - 1;
-    if (FUSED) {
-#pragma unroll
-        for (int j = 0; j < S; ++j) a[j] = x + ((i64)(p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1) * T + t) * s.I;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) v[g] = w.w_ih[d] + ((i64)g * H + wu) * s.I;
-        step_product<S, 4, 2, WIDE>(s.I, a, v, acc);
-    }
-    if (step > 0 || h0) {
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const i64 b = p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1;
-            a[j] = step ? y + ((b * T + before) * s.dirs + d) * H : h0 + ((i64)d * B + b) * H;
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) v[g] = w.w_hh[d] + ((i64)g * H + wu) * H;
-        step_product<S, 4, 2, WIDE>(H, a, v, acc);
-    }
+    auto sequence = [&](int i) -> i64 { return p.b0 + i < B ? p.b0 + i : B - 1; };   // rows behind the last: its values, which are not used
+    auto column = [&](int i) -> uint32_t { return (i >> 4) * H + (p.u0 + (i & 15) < H ? p.u0 + (i & 15) : H - 1); };
+    if (FUSED)
+        step_product<S, 4, WIDE>(
+            s.I, [&](int i) { return x + (sequence(i) * T + t) * s.I; }, w.w_ih[d], [&](int i) { return column(i) * (uint32_t)s.I * 4; }, lds, acc);
+    if (step > 0 || h0)
+        step_product<S, 4, WIDE>(
+            H, [&](int i) { return step ? y + ((sequence(i) * T + before) * s.dirs + d) * H : h0 + ((i64)d * B + sequence(i)) * H; }, w.w_hh[d],
+            [&](int i) { return column(i) * (uint32_t)H * 4; }, lds, acc);
     float sum[S][4];
     step_join<S, 4>(acc, lds, sum);
     if (u >= H) return;
@@ -432,13 +457,13 @@ __global__ __launch_bounds__(256) void lstm_transpose_kernel(int H, Weights w, f
 
 // One step back; step = T - 1 .. 0, and -1 for the gradient of h0.  dc: gradient of the cell between steps, of c0 in the end.
 template <int S, bool WIDE>
-__global__ __launch_bounds__(256) void lstm_step_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0,
-                                                             const float* __restrict__ gates, const float* __restrict__ cells, const float* __restrict__ gy,
-                                                             const float* __restrict__ ghn, const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
-    __shared__ float lds[step_floats<S, 1>()];
+__global__ __launch_bounds__(256, 3) void lstm_step_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0,
+                                                                const float* __restrict__ gates, const float* __restrict__ cells, const float* __restrict__ gy,
+                                                                const float* __restrict__ ghn, const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
+    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 1>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15), uc = u < H ? u : H - 1;
+    const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15), uc = u < H ? u : H - 1;
     float gate[S][4], c[S], c_before[S], dct[S], dh[S];
     i64 at[S], m[S];
 #pragma unroll
@@ -457,13 +482,10 @@ __global__ __launch_bounds__(256) void lstm_step_back_kernel(Shape s, int step, 
         if (gy) dh[j] += gy[((b * T + t) * s.dirs + d) * H + uc];
     }
     f32x4 acc[1][S] = {};
-    if (step < T - 1) {
-        const float *a[S], *v[1];
-#pragma unroll
-        for (int j = 0; j < S; ++j) a[j] = dz + (((i64)d * B + (p.b0 + j * 16 + (lane & 15) < B ? p.b0 + j * 16 + (lane & 15) : B - 1)) * T + after) * 4 * H;
-        v[0] = w_hh_t + ((i64)d * H + (p.u0 + (lane & 15) < H ? p.u0 + (lane & 15) : H - 1)) * 4 * H;
-        step_product<S, 1, 4, WIDE>(4 * H, a, v, acc);
-    }
+    if (step < T - 1)
+        step_product<S, 1, WIDE>(
+            4 * H, [&](int i) { return dz + (((i64)d * B + (p.b0 + i < B ? p.b0 + i : B - 1)) * T + after) * 4 * H; }, w_hh_t + (i64)d * H * 4 * H,
+            [&](int i) { return (uint32_t)(p.u0 + i < H ? p.u0 + i : H - 1) * 16 * H; }, lds, acc);
     float sum[S][1];
     step_join<S, 1>(acc, lds, sum);
     if (u >= H) return;
@@ -507,12 +529,9 @@ int tile_for(i64 m, i64 n) { return cdiv(m, 128) * cdiv(n, 128) >= 512 ? 128 : 6
         else hipLaunchKernelGGL((kernel<64, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                           \
     } while (0)
 
-// 16-sequence blocks of a step's workgroup: as many (up to 4) as leave 256 workgroups
-int step_blocks(const Shape& s) {
-    for (int S = 4; S > 1; S >>= 1)
-        if (cdiv(s.B, 16 * S) * cdiv(s.H, 16) * s.dirs >= 256) return S;
-    return 1;
-}
+// 16-sequence blocks of a step's workgroup: two where that leaves every CU a workgroup.  More would take registers and LDS from a third
+// workgroup on a CU (4 blocks: 12.3 against 11.3 us at 512 sequences of 256 units, the same at 4,096)
+int step_blocks(const Shape& s) { return cdiv(s.B, 32) * cdiv(s.H, 16) * s.dirs >= 256 ? 2 : 1; }
 
 struct Split { int tile, parts, per_part; };
 // the sum over m of the weights' gradients, in parts: about 768 workgroups (3 a CU), and sums of no more than 4,096 products in a row
@@ -542,7 +561,7 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     if (!l) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
     Weights w = {};
-    bool hidden_wide = l->hidden % 16 == 0 && aligned(y) && aligned(h0), input_wide = l->input % 16 == 0 && aligned(x);
+    bool hidden_wide = l->hidden % 4 == 0 && aligned(y) && aligned(h0), input_wide = l->input % 4 == 0 && aligned(x);
     for (int d = 0; d < l->directions; ++d) {
         w.w_ih[d] = l->w_ih[d]; w.w_hh[d] = l->w_hh[d]; w.b_ih[d] = l->b_ih[d]; w.b_hh[d] = l->b_hh[d];
         if (!w.w_ih[d] || !w.w_hh[d] || !w.b_ih[d] || !w.b_hh[d]) return refuse(who, "NULL weight");
@@ -557,7 +576,8 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     const i64 M = l->batch * l->steps, N = 4ll * s.H, all = s.dirs * M * s.H;
     if (!fused) {
         const int tile = tile_for(M, N * s.dirs);
-        DSP_TILES(lstm_inputs_kernel, tile, input_wide, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
+        const bool fast = input_wide && s.I % kStep == 0;   // a line's last 16 values are all its own
+        DSP_TILES(lstm_inputs_kernel, tile, fast, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
     }
     const int S = step_blocks(s);
     const bool wide = hidden_wide && (!fused || input_wide);
@@ -569,8 +589,7 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
         if (fused) { if (wide) DSP_STEP(S, true, true); else DSP_STEP(S, false, true); }                     \
         else { if (wide) DSP_STEP(S, true, false); else DSP_STEP(S, false, false); }                         \
     } while (0)
-        if (S == 4) DSP_STEP_OF(4);
-        else if (S == 2) DSP_STEP_OF(2);
+        if (S == 2) DSP_STEP_OF(2);
         else DSP_STEP_OF(1);
 #undef DSP_STEP_OF
 #undef DSP_STEP
@@ -623,12 +642,11 @@ int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x,
     if (s.B) {
         hipLaunchKernelGGL(lstm_transpose_kernel, dim3((unsigned)cdiv(s.H, 32), (unsigned)cdiv(4 * s.H, 32), dirs), dim3(256), 0, q, s.H, w, wt);
         const int S = step_blocks(s);
-        const bool wide = s.H % 4 == 0;   // 4H in steps of 16, from the workspace
+        const bool wide = s.H % 4 == 0;
         const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * dirs));
         for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step) {
 #define DSP_BACK(S, W) hipLaunchKernelGGL((lstm_step_back_kernel<S, W>), grid, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0)
-            if (S == 4) { if (wide) DSP_BACK(4, true); else DSP_BACK(4, false); }
-            else if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
+            if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
             else { if (wide) DSP_BACK(1, true); else DSP_BACK(1, false); }
 #undef DSP_BACK
         }
