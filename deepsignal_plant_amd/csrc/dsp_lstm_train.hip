@@ -272,6 +272,208 @@ __device__ __forceinline__ float tanh_of(float x) {
     return copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e), x);
 }
 
+// ---- the recurrence of up to 128 units: all steps in one launch --------------------------------------------------------------
+// The recurrent weights of a direction fit a workgroup's registers then (256 KB of 512): a workgroup takes 4 sequences of one
+// direction through all steps, h (forward) or dz (backward) passing through LDS from step to step.  v_mfma_f32_4x4x1 makes 4
+// sequences by 64 columns of one k, the whole of its work useful where the 16 rows of the larger ones would be mostly padding: its
+// 16 blocks all take the same 4 x 1 of A (broadcast from block `k mod 16`, so one register of A serves 16 k) and 4 columns of W
+// each.  What bounds it is the matrix instructions' time (2,048 cycles a step at 128 units) and, behind them, one turn through LDS
+// and the gates.  A launch per step (below) costs 4.5 us instead, at any size: 32 sequences of 128 units, 256 steps: 1.15 ms.
+//
+// N: 16s of units that the registers are for (8, 4 or 2); units beyond H have weights of zero.
+constexpr int kWholeUnits = 128;
+
+// acc[0] = sum over k of A[4][k] W[k][lane]; a: k x 4 in LDS, 16 N values of k
+template <int N> __device__ __forceinline__ f32x4 whole_product(const float* a, const float (&w)[16 * N]) {
+    const int lane = threadIdx.x & 63;
+    f32x4 acc[4] = {};
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a[i * 64 + lane];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#define DSP_K(b) acc[b & 3] = __builtin_amdgcn_mfma_f32_4x4x1f32(v[i], w[i * 16 + b], acc[b & 3], 4, b, 0)
+        DSP_K(0); DSP_K(1); DSP_K(2); DSP_K(3); DSP_K(4); DSP_K(5); DSP_K(6); DSP_K(7);
+        DSP_K(8); DSP_K(9); DSP_K(10); DSP_K(11); DSP_K(12); DSP_K(13); DSP_K(14); DSP_K(15);
+#undef DSP_K
+    }
+    return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+// x[i] of 16-lane row r -> x[r] of row i: what a lane has for 4 sequences becomes what it has for 4 gates
+__device__ __forceinline__ void turn(f32x4& x) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(x[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {   // halves: rows 2 and 3 of v[i] against rows 0 and 1 of v[i + 2]
+        const u32x2 y = __builtin_amdgcn_permlane32_swap(v[i], v[i + 2], false, false);
+        v[i] = y[0];
+        v[i + 2] = y[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {   // rows 1 and 3 of v[i] against rows 0 and 2 of v[i + 1]
+        const u32x2 y = __builtin_amdgcn_permlane16_swap(v[i], v[i + 1], false, false);
+        v[i] = y[0];
+        v[i + 1] = y[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+}
+
+// A wave for every 16 units: in the product lane = gate x 16 + unit and 4 sequences a lane, then lane = sequence x 16 + unit and 4 gates.
+template <int N>
+__global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights weights, const float* __restrict__ h0, const float* __restrict__ c0, float* gates, float* cells,
+                                                            float* h_before, float* __restrict__ y, float* __restrict__ hn, float* __restrict__ cn, int save) {
+    __shared__ __attribute__((aligned(16))) float lds[N * 16 * 64 > 2 * N * 64 ? N * 16 * 64 : 2 * N * 64];
+    const int B = s.B, T = s.T, H = s.H, d = blockIdx.x % s.dirs, b0 = blockIdx.x / s.dirs * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, unit = wave * 16 + (lane & 15), part = lane >> 4;
+    const bool real = unit < H;
+    const int uc = real ? unit : H - 1;
+    // the weights of column (gate part, unit): a row of W_hh, which other lanes load in whole lines
+    float w[16 * N];
+    {
+        const float* w_hh = weights.w_hh[d];
+        float* mine = lds + wave * 64 * 16;   // 64 rows of 16 values of k
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {   // 4 rows at a time
+                const int row = j * 4 + (lane >> 4), k = i * 16 + (lane & 15), u = wave * 16 + (row & 15);
+                mine[row * 16 + ((lane & 15) ^ (row & 15))] = u < H && k < H ? w_hh[((i64)(row >> 4) * H + u) * H + k] : 0.0f;
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[i * 16 + e] = mine[lane * 16 + (e ^ (lane & 15))];
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    const i64 b = b0 + part < B ? b0 + part : B - 1;   // the lane's sequence behind the turn
+    const i64 at = ((i64)d * B + b) * H + uc, first = ((i64)d * B + b) * T;
+    const bool store = real && b0 + part < B;
+    i64 in[4];   // rows of the 4 sequences in the product
+#pragma unroll
+    for (int r = 0; r < 4; ++r) in[r] = (((i64)d * B + (b0 + r < B ? b0 + r : B - 1)) * T * 4 + part) * H + uc;
+    float c = c0 ? c0[at] : 0.0f, h = h0 ? h0[at] : 0.0f;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * N * 64; i += blockDim.x) lds[i] = 0.0f;   // k beyond the units
+    __syncthreads();
+    lds[unit * 4 + part] = real ? h : 0.0f;
+    f32x4 next;
+    const int t0 = d ? T - 1 : 0, dt = d ? -1 : 1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) next[r] = gates[in[r] + (i64)t0 * 4 * H];
+    for (int step = 0; step < T; ++step) {
+        const int t = t0 + step * dt;
+        const i64 m = first + t;
+        const f32x4 z0 = next;
+        if (step + 1 < T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) next[r] = gates[in[r] + (i64)(t + dt) * 4 * H];
+        __syncthreads();   // h of this step is there
+        f32x4 z = whole_product<N>(lds + (step & 1) * N * 64, w) + z0;
+        turn(z);
+        const float i = sigmoid(z[0]), f = sigmoid(z[1]), g = tanh_of(z[2]), o = sigmoid(z[3]);
+        if (save && step == 0 && store) h_before[m * H + unit] = h;
+        c = f * c + i * g;
+        h = o * tanh_of(c);
+        lds[((step & 1) ^ 1) * N * 64 + unit * 4 + part] = real ? h : 0.0f;   // its readers of the step before are behind this step's barrier
+        if (!store) continue;
+        y[((b * T + t) * s.dirs + d) * H + unit] = h;
+        if (save) {
+            float* q = gates + m * 4 * H + unit;
+            q[0] = i;
+            q[H] = f;
+            q[2 * H] = g;
+            q[3 * H] = o;
+            cells[m * H + unit] = c;
+            if (step + 1 < T) h_before[(m + dt) * H + unit] = h;
+        }
+    }
+    if (store) {
+        hn[at] = h;
+        cn[at] = c;
+    }
+}
+
+// Backward: a wave for every gate and 64 units: it multiplies that gate's dz by its rows of W_hh; the 4 gates' sums meet in LDS, where a
+// thread has one unit of one sequence.  M: 64s of units.
+template <int N, int M>
+__global__ __launch_bounds__(256 * M) void lstm_whole_back_kernel(Shape s, Weights weights, const float* __restrict__ c0, const float* __restrict__ gates,
+                                                                  const float* __restrict__ cells, const float* __restrict__ gy, const float* __restrict__ ghn,
+                                                                  const float* __restrict__ gcn, float* __restrict__ dz, float* __restrict__ dc0, float* __restrict__ dh0) {
+    __shared__ float dz_lds[4 * N * 64], sums[4 * 4 * M * 64];   // [gate][k][sequence]; [gate][sequence][unit]
+    const int B = s.B, T = s.T, H = s.H, d = blockIdx.x % s.dirs, b0 = blockIdx.x / s.dirs * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, gate = wave & 3, column = (wave >> 2) * 64 + lane;
+    float w[16 * N];
+    {
+        const float* w_hh = weights.w_hh[d] + (i64)gate * H * H;
+#pragma unroll
+        for (int k = 0; k < 16 * N; ++k) w[k] = k < H && column < H ? w_hh[(i64)k * H + column] : 0.0f;
+    }
+    const int unit = threadIdx.x % (64 * M), seq = threadIdx.x / (64 * M);
+    const bool real = unit < H, store = real && b0 + seq < B;
+    const int uc = real ? unit : H - 1;
+    const i64 b = b0 + seq < B ? b0 + seq : B - 1, at = ((i64)d * B + b) * H + uc, first = ((i64)d * B + b) * T;
+    const int t0 = d ? T - 1 : 0, dt = d ? -1 : 1;   // in time of the recurrence: step k is t0 + k dt
+    for (int i = threadIdx.x; i < 4 * N * 64; i += 256 * M) dz_lds[i] = 0.0f;   // k beyond the units
+    float dc = gcn ? gcn[at] : 0.0f, dh_end = ghn ? ghn[at] : 0.0f;
+    float a[4], next[4], c_next = 0.0f, gy_next = 0.0f, c = cells[(first + t0 + (i64)(T - 1) * dt) * H + uc];
+    auto load = [&](int step) {   // gates, the cell before, gradient of y
+        const int t = t0 + step * dt;
+        const i64 m = first + t;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) next[g] = gates[m * 4 * H + g * H + uc];
+        c_next = step ? cells[(m - dt) * H + uc] : c0 ? c0[at] : 0.0f;
+        gy_next = gy ? gy[((b * T + t) * s.dirs + d) * H + uc] : 0.0f;
+    };
+    load(T - 1);
+    for (int step = T - 1; step >= 0; --step) {
+        const float c_before = c_next, gy_now = gy_next;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) a[g] = next[g];
+        if (step) load(step - 1);
+        __syncthreads();   // dz of the step behind is there
+        f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (step < T - 1) p = whole_product<N>(dz_lds + gate * N * 64, w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[(gate * 4 + r) * M * 64 + column] = p[r];
+        __syncthreads();
+        float dh = gy_now + dh_end;
+        dh_end = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) dh += sums[(g * 4 + seq) * M * 64 + unit];
+        const float tc = tanh_of(c), dcell = dc + dh * a[3] * (1.0f - tc * tc);
+        float q[4];
+        q[0] = dcell * a[2] * a[0] * (1.0f - a[0]);
+        q[1] = dcell * c_before * a[1] * (1.0f - a[1]);
+        q[2] = dcell * a[0] * (1.0f - a[2] * a[2]);
+        q[3] = dh * tc * a[3] * (1.0f - a[3]);
+        dc = dcell * a[1];
+        c = c_before;
+        if (!real) continue;
+        float* out = dz + (first + t0 + (i64)step * dt) * 4 * H + unit;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            dz_lds[(g * N * 16 + unit) * 4 + seq] = q[g];
+            if (store) out[g * H] = q[g];
+        }
+    }
+    if (dh0) {
+        __syncthreads();
+        const f32x4 p = whole_product<N>(dz_lds + gate * N * 64, w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[(gate * 4 + r) * M * 64 + column] = p[r];
+        __syncthreads();
+        float dh = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) dh += sums[(g * 4 + seq) * M * 64 + unit];
+        if (store) dh0[at] = dh;
+    }
+    if (store) dc0[at] = dc;
+}
+
+// ---- the recurrence of more units: a launch per step -------------------------------------------------------------------------
 // A workgroup of 4 waves makes a tile of 16 S sequences by C blocks of 16 columns (forward: the 4 gates of 16 units; backward: 16 units).
 // Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves.  It loads lines of 128 bytes, 8 rows at a
 // time, 32 values of k ahead, and turns them in LDS of its own into what v_mfma_f32_16x16x4 takes (a lane's 4 consecutive k of one
@@ -579,6 +781,13 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
         const bool fast = input_wide && s.I % kStep == 0;   // a line's last 16 values are all its own
         DSP_TILES(lstm_inputs_kernel, tile, fast, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
     }
+    if (!fused && s.H <= kWholeUnits) {
+        const dim3 grid((unsigned)(cdiv(s.B, 4) * s.dirs)), block(64 * (unsigned)cdiv(s.H, 16));
+        if (s.H > 64) hipLaunchKernelGGL(lstm_whole_kernel<8>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
+        else if (s.H > 32) hipLaunchKernelGGL(lstm_whole_kernel<4>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
+        else hipLaunchKernelGGL(lstm_whole_kernel<2>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
+        return launched(who);
+    }
     const int S = step_blocks(s);
     const bool wide = hidden_wide && (!fused || input_wide);
     const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * s.dirs));
@@ -640,15 +849,22 @@ int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x,
     float* part = (float*)ws;
     hipStream_t q = (hipStream_t)stream;
     if (s.B) {
-        hipLaunchKernelGGL(lstm_transpose_kernel, dim3((unsigned)cdiv(s.H, 32), (unsigned)cdiv(4 * s.H, 32), dirs), dim3(256), 0, q, s.H, w, wt);
-        const int S = step_blocks(s);
-        const bool wide = s.H % 4 == 0;
-        const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * dirs));
-        for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step) {
+        if (s.H <= kWholeUnits) {
+            const dim3 grid((unsigned)(cdiv(s.B, 4) * dirs));
+            if (s.H > 64) hipLaunchKernelGGL((lstm_whole_back_kernel<8, 2>), grid, dim3(512), 0, q, s, w, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0);
+            else if (s.H > 32) hipLaunchKernelGGL((lstm_whole_back_kernel<4, 1>), grid, dim3(256), 0, q, s, w, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0);
+            else hipLaunchKernelGGL((lstm_whole_back_kernel<2, 1>), grid, dim3(256), 0, q, s, w, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0);
+        } else {
+            hipLaunchKernelGGL(lstm_transpose_kernel, dim3((unsigned)cdiv(s.H, 32), (unsigned)cdiv(4 * s.H, 32), dirs), dim3(256), 0, q, s.H, w, wt);
+            const int S = step_blocks(s);
+            const bool wide = s.H % 4 == 0;
+            const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * dirs));
+            for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step) {
 #define DSP_BACK(S, W) hipLaunchKernelGGL((lstm_step_back_kernel<S, W>), grid, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0)
-            if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
-            else { if (wide) DSP_BACK(1, true); else DSP_BACK(1, false); }
+                if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
+                else { if (wide) DSP_BACK(1, true); else DSP_BACK(1, false); }
 #undef DSP_BACK
+            }
         }
         if (dx) {
             const int tile = tile_for(M, s.I);
