@@ -87,7 +87,8 @@ __global__ __launch_bounds__(256) void embed_grad_small_kernel(i64 n, i64 per_bl
     extern __shared__ __attribute__((aligned(16))) float table[];
     const int dim = vecs * VEC, groups = blockDim.x >> log_lanes, cells = vocab * dim;
     const int lane = threadIdx.x & ((1 << log_lanes) - 1), group = threadIdx.x >> log_lanes;
-    for (int i = threadIdx.x; i < cells * groups; i += blockDim.x) table[i] = 0.0f;
+    for (int i = threadIdx.x; i < cells * groups / 4; i += blockDim.x) ((f32x4*)table)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (threadIdx.x < (cells * groups & 3)) table[cells * groups - 1 - threadIdx.x] = 0.0f;
     __syncthreads();
     const i64 from = (i64)blockIdx.x * per_block, to = from + per_block < n ? from + per_block : n;
     for (i64 r = from + group; r < to; r += 4 * groups) {
@@ -108,10 +109,27 @@ __global__ __launch_bounds__(256) void embed_grad_small_kernel(i64 n, i64 per_bl
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < cells; i += blockDim.x) {
-        const float* cell = table + (i64)(i / dim) * groups * dim + i % dim;
+    // the groups' tables joined: as many threads a cell as there are, each a range of the groups.  Rows begin in the same bank, so
+    // every row starts at a group of its own.
+    __shared__ float sums[256];
+    const int each = cells < (int)blockDim.x ? blockDim.x / cells : 1, per = (groups + each - 1) / each;
+    for (int i0 = 0; i0 < cells; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x % cells, range = threadIdx.x / cells;   // cells >= blockDim: range 0
         float s = 0.0f;
-        for (int k = 0; k < groups; ++k) s += cell[k * dim];
+        if (i < cells && range < each) {
+            const int v = i / dim, to = (range + 1) * per < groups ? (range + 1) * per : groups;
+            const float* row = table + (i64)v * groups * dim + i % dim;
+#pragma unroll 8
+            for (int k = range * per; k < to; ++k) s += row[((k + v) & (groups - 1)) * dim];
+        }
+        if (each > 1) {
+            sums[threadIdx.x] = s;
+            __syncthreads();
+            s = 0.0f;
+            if ((int)threadIdx.x < cells)
+                for (int r = 0; r < each; ++r) s += sums[r * cells + threadIdx.x];
+        }
+        if (i >= cells || range) continue;
         if (part) part[(i64)blockIdx.x * cells + i] = s;
         else dw[i] = from_f32<T>(s * scale);
     }
@@ -252,7 +270,7 @@ template <class T> __global__ __launch_bounds__(256) void embed_zero_kernel(i64 
     for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < n; i += (i64)gridDim.x * 256) dw[i] = T{};
 }
 
-// A group of lanes walks one chunk of the sorted order for the columns that its lanes hold (blockIdx.y: 64 accesses of columns).
+// A group of lanes walks one chunk of the sorted order for the columns that its lanes hold (64 accesses of columns at most).
 // part[chunk][0]: the sum of the run that reaches into the chunk from before; part[chunk][1]: of the run that begins here
 // and goes on behind it.
 template <class T, int VEC>
@@ -261,8 +279,9 @@ __global__ __launch_bounds__(256) void embed_grad_walk_kernel(i64 n, int chunk, 
                                                               float* __restrict__ part, T* __restrict__ dw) {
     typedef Vec<T, VEC> V;
     typedef Vec<float, VEC> F;
-    const i64 c = (i64)blockIdx.x * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
-    const int v = blockIdx.y * 64 + (threadIdx.x & ((1 << log_lanes) - 1));
+    const int slabs = (vecs + 63) >> 6;   // the parts of a row are neighbours, so that it is read at about one time
+    const i64 c = (i64)(blockIdx.x / slabs) * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
+    const int v = blockIdx.x % slabs * 64 + (threadIdx.x & ((1 << log_lanes) - 1));
     const i64 from = c * chunk, to = from + chunk < n ? from + chunk : n;
     if (from >= n || v >= vecs) return;
     const int dim = vecs * VEC;
@@ -271,16 +290,26 @@ __global__ __launch_bounds__(256) void embed_grad_walk_kernel(i64 n, int chunk, 
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-    for (i64 i = from; i < to; i += 4) {
-        uint32_t k[4];
-        V x[4];
+    constexpr int AHEAD = 8;   // rows of the gradient on their way; which ones they are is read 8 rows before
+    uint32_t k[AHEAD], next_k[AHEAD], next_p[AHEAD];
+    auto read = [&](i64 i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            k[j] = i + j < to ? key[i + j] : (uint32_t)vocab;
-            if (k[j] < (uint32_t)vocab) x[j] = ((const V*)g)[(i64)pos[i + j] * vecs + v];
+        for (int j = 0; j < AHEAD; ++j) {
+            next_k[j] = i + j < to ? key[i + j] : (uint32_t)vocab;
+            next_p[j] = i + j < to ? pos[i + j] : 0;
         }
+    };
+    read(from);
+    for (i64 i = from; i < to; i += AHEAD) {
+        V x[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < AHEAD; ++j) {
+            k[j] = next_k[j];
+            if (k[j] < (uint32_t)vocab) x[j] = ((const V*)g)[(i64)next_p[j] * vecs + v];
+        }
+        read(i + AHEAD);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
             if (i + j >= to) break;
             if (k[j] != run) {
                 if (run < (uint32_t)vocab) {   // a run ends inside the chunk
@@ -321,38 +350,47 @@ __global__ __launch_bounds__(256) void embed_grad_walk_kernel(i64 n, int chunk, 
     }
 }
 
-// A block per chunk in which a run begins that goes on behind it (the others end at once): the run's last chunk is found by
-// bisection, 4 parts of the block add a quarter of its partial sums each, then their four sums are joined in order.
-template <class T>
-__global__ __launch_bounds__(256) void embed_grad_join_kernel(i64 n, int chunk, i64 chunks, int dim, const uint32_t* __restrict__ key, int vocab,
+// A block per chunk in which a run begins that goes on behind it (the others end at once) and 64 x VEC columns: the run's last chunk is found
+// by bisection; groups of lanes, VEC columns a lane, add a range of its partial sums each, then their sums are joined in order.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void embed_grad_join_kernel(i64 n, int chunk, i64 chunks, int vecs, int log_lanes, const uint32_t* __restrict__ key, int vocab,
                                                               float scale, const float* __restrict__ part, T* __restrict__ dw) {
-    __shared__ float sums[4][64];
+    typedef Vec<float, VEC> F;
+    __shared__ F sums[256];
     const i64 c = blockIdx.x, from = c * chunk, to = from + chunk;
     if (to >= n) return;
-    const uint32_t run = key[to];
-    if (run >= (uint32_t)vocab || key[to - 1] != run) return;
-    if (key[from] == run && from > 0 && key[from - 1] == run) return;   // it began in an earlier chunk
+    const uint32_t run = key[to], last = key[to - 1], start = key[from], before = from > 0 ? key[from - 1] : 0xffffffffu;
+    if (run >= (uint32_t)vocab || last != run || (start == run && before == run)) return;   // no run goes on, or it began in an earlier chunk
     i64 lo = c + 1, hi = chunks;   // chunks lo - 1 and before begin with the run (or hold its beginning), hi and behind do not
     while (lo < hi) {
         const i64 mid = (lo + hi) >> 1;
         if (key[mid * chunk] == run) lo = mid + 1;
         else hi = mid;
     }
-    const i64 count = lo - (c + 1), quarter = (count + 3) / 4;   // partial sums behind the first
-    const int q = threadIdx.x >> 6;
-    for (int col0 = 0; col0 < dim; col0 += 64) {
-        const int col = col0 + (threadIdx.x & 63);
-        float s = 0.0f;
-        if (col < dim) {
-            if (q == 0) s = part[(c * 2 + 1) * dim + col];
-            const i64 end = (q + 1) * quarter < count ? (q + 1) * quarter : count;
-            for (i64 i = q * quarter; i < end; ++i) s += part[(c + 1 + i) * 2 * dim + col];
+    const int lanes = 1 << log_lanes, groups = 256 >> log_lanes, group = threadIdx.x >> log_lanes, v = blockIdx.y * 64 + (threadIdx.x & (lanes - 1));
+    const i64 count = lo - (c + 1), per = (count + groups - 1) / groups;   // partial sums behind the first
+    F s;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s.v[e] = 0.0f;
+    if (v < vecs) {
+        const F* p = (const F*)part + v;
+        if (group == 0) s = p[(c * 2 + 1) * vecs];
+        const i64 end = (group + 1) * per < count ? (group + 1) * per : count;
+#pragma unroll 8
+        for (i64 i = group * per; i < end; ++i) {
+            const F x = p[(c + 1 + i) * 2 * vecs];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s.v[e] += x.v[e];
         }
-        sums[q][threadIdx.x & 63] = s;
-        __syncthreads();
-        if (q == 0 && col < dim) dw[(i64)run * dim + col] = from_f32<T>((sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x]) * scale);
-        __syncthreads();
     }
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    if (group || v >= vecs) return;
+    for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s.v[e] += sums[g * lanes + threadIdx.x].v[e];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[(i64)run * vecs * VEC + v * VEC + e] = from_f32<T>(s.v[e] * scale);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
@@ -374,8 +412,8 @@ bool small_table(i64 vocab, i64 dim) {
     return groups_that_fit(vocab, dim, wave) == wave;
 }
 int type_size(int dt) { return dt == DSP_FT_F32 ? 4 : 2; }
-i64 small_blocks(i64 n, int groups) {
-    const i64 b = cdiv(n, (i64)groups * 16);
+i64 small_blocks(i64 n, int groups) {   // 4 tokens a group at least, the loads that it has under way at once
+    const i64 b = cdiv(n, (i64)groups * 4);
     return b < 1 ? 1 : b > 512 ? 512 : b;
 }
 int key_bits(i64 vocab) {   // keys 0 .. vocab
@@ -419,7 +457,8 @@ template <class T, int VEC>
 void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, const void* g, int vocab, int pad, float scale, void* dw, char* ws) {
     const int vecs = dim / VEC, ll = log2_lanes(vecs);
     if (small_table(vocab, dim)) {
-        const int cells = vocab * dim, use = groups_that_fit(vocab, dim, 256 >> ll);
+        // workgroups of one wave until there are 512 of them (13,312 x 16 x 4: half the tables to clear and to join), then of 4
+        const int cells = vocab * dim, use = groups_that_fit(vocab, dim, (n > 512 * 4 * (64 >> ll) ? 256 : 64) >> ll);
         const i64 blocks = small_blocks(n, use);
         float* part = blocks > 1 ? (float*)ws : nullptr;
         hipLaunchKernelGGL((embed_grad_small_kernel<T, VEC>), dim3((unsigned)blocks), dim3(use << ll), (size_t)cells * use * 4, s, n, cdiv(n, blocks), vecs, ll,
@@ -444,9 +483,12 @@ void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, cons
         pos = po;
     }
     float* part = (float*)(ws + p.part);
-    hipLaunchKernelGGL((embed_grad_walk_kernel<T, VEC>), dim3((unsigned)cdiv(p.chunks, 256 >> ll), (unsigned)cdiv(vecs, 64)), dim3(256), 0, s, n, p.chunk, vecs,
+    hipLaunchKernelGGL((embed_grad_walk_kernel<T, VEC>), dim3((unsigned)(cdiv(p.chunks, 256 >> ll) * cdiv(vecs, 64))), dim3(256), 0, s, n, p.chunk, vecs,
                        ll, key, pos, (const T*)g, vocab, scale, part, (T*)dw);
-    hipLaunchKernelGGL((embed_grad_join_kernel<T>), dim3((unsigned)p.chunks), dim3(256), 0, s, n, p.chunk, p.chunks, dim, key, vocab, scale, part, (T*)dw);
+    constexpr int JOIN = VEC < 4 ? VEC : 4;   // columns a lane
+    const int jv = dim / JOIN;
+    hipLaunchKernelGGL((embed_grad_join_kernel<T, JOIN>), dim3((unsigned)p.chunks, (unsigned)cdiv(jv, 64)), dim3(256), 0, s, n, p.chunk, p.chunks, jv, log2_lanes(jv),
+                       key, vocab, scale, part, (T*)dw);
 }
 
 const char* bad_embedding(i64 n, i64 vocab, i64 dim, int dt, int ft) {

@@ -92,6 +92,12 @@ def test_embedding_lengths_and_tables(ops, n, rows):
     check_embedding(ops, tokens_of(n, rows, torch.int32), table(rows, 4))
 
 
+@pytest.mark.parametrize("rows,dim,n", [(16, 4, 852000), (64, 4, 200000), (63, 3, 150001), (60, 256, 40000), (256, 1, 140000), (300, 64, 60000)])
+def test_embedding_many_tokens_of_small_tables(ops, rows, dim, n):
+    check_embedding(ops, tokens_of(n, rows, torch.int32), table(rows, dim))
+    check_embedding(ops, tokens_of(n, rows, torch.int32), table(rows, dim, BF16), scale=3.0)
+
+
 @pytest.mark.parametrize("rows,dim", [(16, 4), (5000, 24), (300000, 8), (2 ** 21, 1)])
 def test_embedding_one_token_takes_all(ops, rows, dim):
     """a run over every chunk of the sorted order, and all but a few"""
