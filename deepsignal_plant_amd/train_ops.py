@@ -15,6 +15,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
+from operator import attrgetter
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -283,6 +285,9 @@ def cross_entropy(logits, labels, weight=None, ignore_index=-100, reduction="mea
 
 
 # ---- the norm of many gradients -----------------------------------------------------------------------------------------------
+_dtype, _layout, _shape = attrgetter("dtype"), attrgetter("layout"), attrgetter("shape")
+
+
 def _is_dense(t):
     """whether the values fill one piece of memory, in whatever order"""
     if t.is_contiguous():
@@ -295,23 +300,27 @@ def _is_dense(t):
     return True
 
 
+# lists of hundreds of tensors go through map(): a loop in Python costs as much as the kernels
 def _check_grads(who, grads):
     """the index of their GPU"""
     for g in grads:
-        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided:
+        if not isinstance(g, torch.Tensor):
             raise ValueError("%s: gradients must be dense tensors" % who)
-        if g.dtype not in _FLOAT:
-            raise ValueError("%s: gradients must be float32, bfloat16 or float16, got %s" % (who, g.dtype))
-    return _one_gpu(who, *grads)
+    if set(map(_layout, grads)) != {torch.strided}:
+        raise ValueError("%s: gradients must be dense tensors" % who)
+    for dtype in set(map(_dtype, grads)):
+        if dtype not in _FLOAT:
+            raise ValueError("%s: gradients must be float32, bfloat16 or float16, got %s" % (who, dtype))
+    return _one_gpu(who, *grads) if len(set(map(torch.Tensor.get_device, grads))) > 1 else _one_gpu(who, grads[0])
 
 
 class _Pieces(object):
     """where tensors lie: addresses, numbers of values, types, and (start, end) of those that are not empty in order"""
 
-    def __init__(self, tensors):
-        self.ptrs = [t.data_ptr() for t in tensors]
-        self.numels = [t.numel() for t in tensors]
-        self.types = [_FLOAT[t.dtype] for t in tensors]
+    def __init__(self, tensors, like=None):   # like: another's numbers of values
+        self.ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
+        self.numels = array("q", map(torch.Tensor.numel, tensors)) if like is None else like.numels
+        self.types = array("i", map(_FLOAT.__getitem__, map(_dtype, tensors)))
         self.spans = sorted([(p, p + n * (2 if t else 4)) for p, n, t in zip(self.ptrs, self.numels, self.types) if n])
 
     def check_apart(self, who):
@@ -322,6 +331,8 @@ class _Pieces(object):
             end = stop
 
     def check_apart_from(self, who, others):
+        if not self.spans or not others.spans or self.spans[0][0] >= others.spans[-1][1] or others.spans[0][0] >= self.spans[-1][1]:
+            return
         other = iter(others.spans)
         at = next(other, None)
         for start, end in self.spans:
@@ -332,13 +343,12 @@ class _Pieces(object):
 
 
 def _run_clip(dev, like, grads, outs, max_norm):
-    n, L = len(grads.ptrs), nat.lib()
-    ptr, i32 = ctypes.c_void_p * n, ctypes.c_int32 * n
-    numels = (ctypes.c_int64 * n)(*grads.numels)
+    n, L, numels = len(grads.ptrs), nat.lib(), grads.numels.buffer_info()[0]
     norm = like.new_empty((), dtype=torch.float32)
     ws = _workspace(like, L.dsp_clip_workspace(n, numels))
-    _call(dev, L.dsp_clip_grad_norm, n, ptr(*grads.ptrs), numels, i32(*grads.types), None if outs is None else ptr(*outs.ptrs),
-          None if outs is None else i32(*outs.types), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    at = lambda pieces, name: None if pieces is None else getattr(pieces, name).buffer_info()[0]
+    _call(dev, L.dsp_clip_grad_norm, n, at(grads, "ptrs"), numels, at(grads, "types"), at(outs, "ptrs"), at(outs, "types"), max_norm, norm.data_ptr(),
+          ws.data_ptr(), ws.numel())
     return norm
 
 
@@ -374,12 +384,20 @@ def clip_grad_norm(grads, max_norm, out=None):
     out = [g.new_empty(g.shape) for g in grads] if out is None else list(out)
     if len(out) != len(grads):
         raise ValueError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
-    _one_gpu(who, grads[0], *out)
-    for g, o in zip(grads, out):
-        if o.shape != g.shape or not o.is_contiguous() or (o.dtype is not g.dtype and o.dtype is not torch.float32):
-            raise ValueError("clip_grad_norm: an output must be contiguous, of its gradient's shape, and of its type or float32")
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    ins, outs = _Pieces(grads), _Pieces(out)
+    for o in out:
+        if not isinstance(o, torch.Tensor):
+            raise ValueError("clip_grad_norm: expected a tensor, got %s" % type(o).__name__)
+    if set(map(torch.Tensor.get_device, out)) != {dev}:
+        _one_gpu(who, grads[0], *out)
+    if list(map(_shape, grads)) != list(map(_shape, out)) or not all(map(torch.Tensor.is_contiguous, out)):
+        raise ValueError("clip_grad_norm: an output must be contiguous and of its gradient's shape")
+    for g, o in set(zip(map(_dtype, grads), map(_dtype, out))):
+        if o is not g and o is not torch.float32:
+            raise ValueError("clip_grad_norm: an output must be of its gradient's type or float32")
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]
+    ins = _Pieces(grads)
+    outs = _Pieces(out, ins)
     outs.check_apart(who)
     outs.check_apart_from(who, ins)
     norm = _run_clip(dev, grads[0], ins, outs, max_norm)
