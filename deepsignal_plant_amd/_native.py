@@ -290,6 +290,9 @@ def lib():
             ("dsp_lstm_forward", I32, [P] * 9 + [P, I32]),
             ("dsp_lstm_workspace", I64, [P]),
             ("dsp_lstm_backward", I32, [P] * 13 + [P, I64]),
+            ("dsp_linear_forward", I32, [P, I64, I64, I64, P, P, P, P]),
+            ("dsp_linear_workspace", I64, [I64, I64, I64]),
+            ("dsp_linear_backward", I32, [P, I64, I64, I64] + [P] * 7 + [I64]),
             ("dsp_cross_entropy_workspace", I64, [I64]),
             ("dsp_cross_entropy_forward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, P, P, I64]),
             ("dsp_cross_entropy_backward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, I32, P]),

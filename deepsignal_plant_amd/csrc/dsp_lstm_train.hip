@@ -14,173 +14,18 @@
 //
 // Layouts: x [B][T][I], y [B][T][dirs H], states [dirs][B][H]; gates and their gradients [dirs][B][T][4H]; cells and the h before
 // each step [dirs][B][T][H].  So the products over all steps are plain: a row is m = b T + t.
-#include "dsp_ops.h"
+#include "dsp_products.h"
 
 using namespace dsp;
 
 namespace {
-
-// ---- the products over all steps -----------------------------------------------------------------------------------------
-// C(m, n) = sum over k of A(m, k) B(n, k).  A workgroup of 4 waves makes a tile of TILE x TILE, a wave a quarter of it as 32 x 32
-// blocks of v_mfma_f32_32x32x2.  16 values of k are staged in LDS at a time, the next 16 on their way in registers and the ones
-// before them in the other half of LDS: one barrier per 16.  A lane's 4 values of k are consecutive (lane group q takes k =
-// 4q + j for instruction j): the order of k is the same for both operands, so any is right.
-//
-// On this device vector instructions take their time from the fp32 matrix instructions, so the loop has next to none: where
-// sizes and addresses allow (FAST), the operands come by buffer loads whose lane offsets are made once and whose descriptors
-// end with the operand: what lies behind it reads as zeros.  Otherwise (an input size of 7) every value is guarded.
-constexpr int kStep = 16;
-
-struct Matrix {   // row-major, `lines` lines of `ld` values
-    const float* p;
-    int lines, ld;
-};
-
-// ALONG_K: a line is a row of the product, k along it.  Else a line is a k, the product's rows along it.
-template <bool ALONG_K, int TILE, bool FAST> struct Stage {
-    static constexpr int kStride = ALONG_K ? kStep + 4 : TILE + 4;
-    static constexpr int kFloats = ALONG_K ? TILE * kStride : kStep * kStride;
-    static constexpr int kLoads = TILE * kStep / 4 / 256, kAcross = ALONG_K ? kStep / 4 : TILE / 4;   // accesses of 4 along a line
-    f32x4 v[kLoads];
-    Matrix m;
-    int row0, k_end;
-    __amdgpu_buffer_rsrc_t rsrc;
-    int lane_at[kLoads];
-    uint32_t at, per_step;
-    __device__ __forceinline__ Stage(const Matrix& matrix, int row, int k0, int k1) : m(matrix), row0(row), k_end(k1) {
-        if (!FAST) return;
-        const float* base = ALONG_K ? m.p + (i64)row0 * m.ld : m.p + (i64)k0 * m.ld + row0;
-        const i64 bytes = ((i64)m.lines * m.ld - (base - m.p)) * 4;
-        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes), 0x00020000);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int j = threadIdx.x + i * 256;
-            lane_at[i] = (j / kAcross * m.ld + j % kAcross * 4) * 4;
-        }
-        at = ALONG_K ? k0 * 4 : 0;
-        per_step = ALONG_K ? kStep * 4 : (uint32_t)m.ld * kStep * 4;
-    }
-    __device__ __forceinline__ void fetch(int k) {
-        if (FAST) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane_at[i], (int)at, 0));
-            at += per_step;
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int j = threadIdx.x + i * 256;
-            const int line = (ALONG_K ? row0 : k) + j / kAcross, on = (ALONG_K ? k : row0) + j % kAcross * 4;
-            const int lines = ALONG_K ? m.lines : k_end, most = ALONG_K ? k_end : m.ld;
-            const float* p = m.p + (i64)line * m.ld + on;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = line < lines && on + e < most ? p[e] : 0.0f;
-        }
-    }
-    __device__ __forceinline__ void put(float* lds) const {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int j = threadIdx.x + i * 256;
-            *(f32x4*)(lds + j / kAcross * kStride + j % kAcross * 4) = v[i];
-        }
-    }
-    // 4 consecutive values of k of one row
-    static __device__ __forceinline__ f32x4 get(const float* lds, int row, int k) {
-        if (ALONG_K) return *(const f32x4*)(lds + row * kStride + k);
-        f32x4 r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = lds[(k + e) * kStride + row];
-        return r;
-    }
-};
-template <bool A_ALONG_K, bool B_ALONG_K, int TILE> constexpr int half_floats() {
-    return Stage<A_ALONG_K, TILE, false>::kFloats + Stage<B_ALONG_K, TILE, false>::kFloats;
-}
-
-// acc[i][j] (block (i, j) of the wave's quarter) += over k in [k0, k1).  f(values of A as they are staged) for every 16 of k
-template <bool A_ALONG_K, bool B_ALONG_K, int TILE, bool FAST, class F>
-__device__ __forceinline__ void product(const Matrix& a, const Matrix& b, int m0, int n0, int k0, int k1, float* lds, f32x16 (&acc)[TILE / 64][TILE / 64], F f) {
-    typedef Stage<A_ALONG_K, TILE, FAST> SA;
-    typedef Stage<B_ALONG_K, TILE, FAST> SB;
-    constexpr int R = TILE / 64, HALF = SA::kFloats + SB::kFloats;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * (TILE / 2) + (lane & 31), wn = (wave & 1) * (TILE / 2) + (lane & 31), kq = (lane >> 5) * 4;
-    if (k0 >= k1) return;
-    SA sa(a, m0, k0, k1);
-    SB sb(b, n0, k0, k1);
-    auto step = [&](int half, int k) {   // 16 values of k from one half of LDS; the next 16 into the other
-        const float *la = lds + half * HALF, *lb = la + SA::kFloats;
-#pragma unroll
-        for (int kk = 0; kk < kStep; kk += 8) {
-            f32x4 fa[R], fb[R];
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                fa[i] = SA::get(la, wm + i * 32, kk + kq);
-                fb[i] = SB::get(lb, wn + i * 32, kk + kq);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-#pragma unroll
-                    for (int j = 0; j < R; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
-        }
-        if (k + kStep < k1) {
-            float* next = lds + (half ^ 1) * HALF;
-            f(sa.v);
-            sa.put(next);
-            sb.put(next + SA::kFloats);
-            if (k + 2 * kStep < k1) {
-                sa.fetch(k + 2 * kStep);
-                sb.fetch(k + 2 * kStep);
-            }
-        }
-        __syncthreads();
-    };
-    sa.fetch(k0);
-    sb.fetch(k0);
-    __syncthreads();   // what used LDS before is done
-    f(sa.v);
-    sa.put(lds);
-    sb.put(lds + SA::kFloats);
-    if (k0 + kStep < k1) {
-        sa.fetch(k0 + kStep);
-        sb.fetch(k0 + kStep);
-    }
-    __syncthreads();
-    for (int k = k0; k < k1; k += 2 * kStep) {
-        step(0, k);
-        if (k + kStep < k1) step(1, k + kStep);
-    }
-}
-// f(m, n, value) for every value of the tile that is inside
-template <int TILE, class F> __device__ __forceinline__ void each(const f32x16 (&acc)[TILE / 64][TILE / 64], int m0, int M, int n0, int N, F f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < TILE / 64; ++i)
-#pragma unroll
-        for (int j = 0; j < TILE / 64; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m0 + (wave >> 1) * (TILE / 2) + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-                const int n = n0 + (wave & 1) * (TILE / 2) + j * 32 + (lane & 31);
-                if (m < M && n < N) f(m, n, acc[i][j][r]);
-            }
-}
-// Workgroups go to the 8 dies in turn, each with an L2 of its own: give each die a contiguous range of the tiles, so that tiles of the same
-// rows (neighbours in it) find them there.
-__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint32_t tiles) {
-    const uint32_t die = block & 7, per = tiles >> 3, more = tiles & 7;
-    return die * per + (die < more ? die : more) + (block >> 3);
-}
-struct Nothing { template <class V> __device__ __forceinline__ void operator()(const V&) const {} };
 
 struct Shape { int B, T, I, H, dirs; };
 struct Weights { const float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
 
 // gates = W_ih x + b_ih + b_hh, all steps
 template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
-    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, TILE>()];
+    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<true, true, TILE>()];
     const int M = s.B * s.T, N = 4 * s.H, n_tiles = (N + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int n0 = tile % (n_tiles * s.dirs), d = n0 / n_tiles, at = (n0 - d * n_tiles) * TILE, m0 = tile / (n_tiles * s.dirs) * TILE;
@@ -192,7 +37,7 @@ template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_in
 
 // dx = sum over directions of dz W_ih
 template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
-    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, false, TILE>()];
+    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<true, false, TILE>()];
     const int M = s.B * s.T, K = 4 * s.H, n_tiles = (s.I + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int n0 = tile % n_tiles * TILE, m0 = tile / n_tiles * TILE;
@@ -206,7 +51,7 @@ template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_in
 template <int TILE, bool FAST>
 __global__ __launch_bounds__(256) void lstm_weight_grad_kernel(Shape s, const float* __restrict__ dz, const float* __restrict__ x, const float* __restrict__ h_before,
                                                                int per_part, float* __restrict__ part) {
-    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<false, false, TILE>()];
+    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<false, false, TILE>()];
     const int M = 4 * s.H, K = s.B * s.T, m_tiles = (M + TILE - 1) / TILE, x_tiles = (s.I + TILE - 1) / TILE, n_tiles = x_tiles + (s.H + TILE - 1) / TILE;
     uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int nt = tile % n_tiles;
@@ -219,22 +64,11 @@ __global__ __launch_bounds__(256) void lstm_weight_grad_kernel(Shape s, const fl
     f32x16 acc[TILE / 64][TILE / 64] = {};
     float* out = part + (i64)dq * M * cols;
     if (nt == 0) {   // these see every dz of their rows once: db on the way
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        product<false, false, TILE, FAST>(a, b, m0, n0, k0, k1, lds, acc, [&](const auto& v) {
-            for (const f32x4& y : v) sum += y;
+        RowSums<TILE> sums;
+        product<false, false, TILE, FAST>(a, b, m0, n0, k0, k1, lds, acc, sums);
+        sums.store(lds, [&](int row, float v) {
+            if (m0 + row < M) out[(i64)(m0 + row) * cols + cols - 1] = v;
         });
-        // a thread has summed 4 rows for the values of k that came to it: rows by access along a line, k by line
-        constexpr int kAcross = TILE / 4, kLines = 256 / kAcross;
-        f32x4* sums = (f32x4*)lds;
-        __syncthreads();
-        sums[threadIdx.x] = sum;
-        __syncthreads();
-        if (threadIdx.x < kAcross) {
-            for (int i = 1; i < kLines; ++i) sum += sums[i * kAcross + threadIdx.x];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (m0 + (int)threadIdx.x * 4 + e < M) out[(i64)(m0 + threadIdx.x * 4 + e) * cols + cols - 1] = sum[e];
-        }
     } else
         product<false, false, TILE, FAST>(a, b, m0, n0, k0, k1, lds, acc, Nothing());
     each<TILE>(acc, m0, M, n0, N, [&](int m, int n, float v) { out[(i64)m * cols + n + (of_x ? 0 : s.I)] = v; });
@@ -325,7 +159,7 @@ __device__ __forceinline__ void turn(f32x4& x) {
 template <int N>
 __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights weights, const float* __restrict__ h0, const float* __restrict__ c0, float* gates, float* cells,
                                                             float* h_before, float* __restrict__ y, float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ __attribute__((aligned(16))) float lds[N * 16 * 64 > 2 * N * 64 ? N * 16 * 64 : 2 * N * 64];
+    __shared__ __attribute__((aligned16(16))) float lds[N * 16 * 64 > 2 * N * 64 ? N * 16 * 64 : 2 * N * 64];
     const int B = s.B, T = s.T, H = s.H, d = blockIdx.x % s.dirs, b0 = blockIdx.x / s.dirs * 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, unit = wave * 16 + (lane & 15), part = lane >> 4;
     const bool real = unit < H;
@@ -589,7 +423,7 @@ template <int S, bool WIDE, bool FUSED>
 __global__ __launch_bounds__(256, 3) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ x, const float* __restrict__ h0,
                                                         const float* __restrict__ c0, float* gates, float* cells, float* h_before, float* y,
                                                         float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 4>()];
+    __shared__ __attribute__((aligned16(16))) float lds[step_floats<S, 4>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
     const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15);
@@ -662,7 +496,7 @@ template <int S, bool WIDE>
 __global__ __launch_bounds__(256, 3) void lstm_step_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0,
                                                                 const float* __restrict__ gates, const float* __restrict__ cells, const float* __restrict__ gy,
                                                                 const float* __restrict__ ghn, const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
-    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 1>()];
+    __shared__ __attribute__((aligned16(16))) float lds[step_floats<S, 1>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
     const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15), uc = u < H ? u : H - 1;
@@ -719,39 +553,12 @@ const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
     if (B * T * (H > I ? H : I) >= (1ll << 37)) return "the layer's activations would not fit any device";
     return nullptr;
 }
-bool aligned(const void* p) { return (size_t)p % 16 == 0; }
-
-// tiles of 128 x 128 where they fill the device twice, else of 64 x 64
-int tile_for(i64 m, i64 n) { return cdiv(m, 128) * cdiv(n, 128) >= 512 ? 128 : 64; }
-#define DSP_TILES(kernel, tile, fast, blocks, s, ...)                                                                                   \
-    do {                                                                                                                                \
-        if (tile == 128 && fast) hipLaunchKernelGGL((kernel<128, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);       \
-        else if (tile == 128) hipLaunchKernelGGL((kernel<128, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);         \
-        else if (fast) hipLaunchKernelGGL((kernel<64, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                  \
-        else hipLaunchKernelGGL((kernel<64, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                           \
-    } while (0)
-
 // 16-sequence blocks of a step's workgroup: two where that leaves every CU a workgroup.  More would take registers and LDS from a third
 // workgroup on a CU (4 blocks: 12.3 against 11.3 us at 512 sequences of 256 units, the same at 4,096)
 int step_blocks(const Shape& s) { return cdiv(s.B, 32) * cdiv(s.H, 16) * s.dirs >= 256 ? 2 : 1; }
 
-struct Split { int tile, parts, per_part; };
-// the sum over m of the weights' gradients, in parts: about 768 workgroups (3 a CU), and sums of no more than 4,096 products in a row
-Split split_of(i64 B, i64 T, i64 I, i64 H, int dirs) {
-    Split q;
-    const i64 M = 4 * H, K = B * T;
-    q.tile = cdiv(M, 128) * (cdiv(I, 128) + cdiv(H, 128)) * dirs * cdiv(K, 512) >= 256 ? 128 : 64;
-    const i64 tiles = cdiv(M, q.tile) * (cdiv(I, q.tile) + cdiv(H, q.tile)) * dirs;
-    i64 parts = cdiv(768, tiles);
-    if (parts > cdiv(K, 256)) parts = cdiv(K, 256);
-    if (parts < cdiv(K, 4096)) parts = cdiv(K, 4096);
-    if (parts < 1) parts = 1;
-    q.per_part = (int)(cdiv(cdiv(K, parts), kStep) * kStep);
-    if (q.per_part < kStep) q.per_part = kStep;
-    q.parts = (int)cdiv(K, q.per_part);
-    if (q.parts < 1) q.parts = 1;
-    return q;
-}
+// the sum over m of the weights' gradients
+Split weight_split(const dsp_lstm_layer* l) { return split_of(l->batch * l->steps, 4 * l->hidden, l->input, l->hidden, l->directions); }
 
 }  // namespace
 
@@ -763,12 +570,12 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     if (!l) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
     Weights w = {};
-    bool hidden_wide = l->hidden % 4 == 0 && aligned(y) && aligned(h0), input_wide = l->input % 4 == 0 && aligned(x);
+    bool hidden_wide = l->hidden % 4 == 0 && aligned16(y) && aligned16(h0), input_wide = l->input % 4 == 0 && aligned16(x);
     for (int d = 0; d < l->directions; ++d) {
         w.w_ih[d] = l->w_ih[d]; w.w_hh[d] = l->w_hh[d]; w.b_ih[d] = l->b_ih[d]; w.b_hh[d] = l->b_hh[d];
         if (!w.w_ih[d] || !w.w_hh[d] || !w.b_ih[d] || !w.b_hh[d]) return refuse(who, "NULL weight");
-        hidden_wide = hidden_wide && aligned(w.w_hh[d]);
-        input_wide = input_wide && aligned(w.w_ih[d]);
+        hidden_wide = hidden_wide && aligned16(w.w_hh[d]);
+        input_wide = input_wide && aligned16(w.w_ih[d]);
     }
     if (l->batch == 0) return DSP_OK;
     const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, l->directions};
@@ -810,7 +617,7 @@ int64_t dsp_lstm_workspace(const dsp_lstm_layer* l) {
     const char* who = "dsp_lstm_workspace";
     if (!l) return refuse(who, "NULL layer");
     if (const char* why = bad_lstm(l->batch, l->steps, l->input, l->hidden, l->directions)) return refuse(who, why);
-    const Split p = split_of(l->batch, l->steps, l->input, l->hidden, l->directions);
+    const Split p = weight_split(l);
     size_t bytes = align256((size_t)l->directions * l->hidden * 4 * l->hidden * 4);                                    // W_hh transposed
     bytes += align256((size_t)l->directions * l->steps * l->batch * 4 * l->hidden * 4);                                // dz
     return (int64_t)(bytes + align256((size_t)p.parts * l->directions * 4 * l->hidden * (l->input + l->hidden + 1) * 4));   // parts of dW and db
@@ -825,13 +632,13 @@ int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x,
     const int dirs = l->directions;
     Weights w = {};
     Grads out = {};
-    bool input_wide = l->input % 4 == 0 && aligned(x);
+    bool input_wide = l->input % 4 == 0 && aligned16(x);
     for (int d = 0; d < dirs; ++d) {
         w.w_ih[d] = l->w_ih[d];
         w.w_hh[d] = l->w_hh[d];
         out.w_ih[d] = g->w_ih[d]; out.w_hh[d] = g->w_hh[d]; out.b_ih[d] = g->b_ih[d]; out.b_hh[d] = g->b_hh[d];
         if (!w.w_ih[d] || !w.w_hh[d] || !out.w_ih[d] || !out.w_hh[d] || !out.b_ih[d] || !out.b_hh[d]) return refuse(who, "NULL weight or gradient");
-        input_wide = input_wide && aligned(w.w_ih[d]);
+        input_wide = input_wide && aligned16(w.w_ih[d]);
     }
     if (l->batch && (!x || !gates || !cells || !dc0)) return refuse(who, "NULL pointer");
     if (!workspace || workspace_bytes < dsp_lstm_workspace(l)) return refuse(who, "workspace too small (dsp_lstm_workspace)");
@@ -839,8 +646,8 @@ int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x,
     const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, dirs};
     const i64 M = (i64)s.B * s.T;
     const float* h_before = cells + dirs * M * s.H;
-    const bool hidden_wide = s.H % 4 == 0 && aligned(cells);
-    const Split p = split_of(l->batch, l->steps, l->input, l->hidden, dirs);
+    const bool hidden_wide = s.H % 4 == 0 && aligned16(cells);
+    const Split p = weight_split(l);
     char* ws = (char*)workspace;
     float* wt = (float*)ws;
     ws += align256((size_t)dirs * s.H * 4 * s.H * 4);

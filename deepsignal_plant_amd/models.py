@@ -4,6 +4,10 @@ Same constructor arguments, same state_dict keys/shapes, same call signature and
 (logits, softmax) as the reference class; the arithmetic runs in libdsp_amd.so (hand-written HIP, fp32
 MFMA) through the C ABI in include/dsp_amd.h.  torch is used only for device memory, streams and
 checkpoint I/O.  There is no CPU path: forward() on a non-GPU tensor or without the library raises.
+
+train() makes the parameters leaves of torch's autograd on the GPU and forward() differentiable (training.py over
+train_ops.py), as the reference's `train` uses its class (train.py:75-119); eval() hands the trained values to the inference
+kernels.
 """
 from __future__ import annotations
 
@@ -13,6 +17,7 @@ from collections import OrderedDict
 import torch
 
 from . import _native as nat
+from . import training
 
 _DT = {torch.float32: nat.DT_F32, torch.uint8: nat.DT_U8, torch.uint16: nat.DT_U16, torch.int32: nat.DT_I32}
 
@@ -52,7 +57,8 @@ class ModelBiLSTM(object):
         self._params = OrderedDict((k, torch.zeros(shp, dtype=torch.float32)) for k, shp in self._spec)
         self._handle = None
         self._precision = None
-        self._training = True
+        self._leaves = None        # name -> leaf tensor on the GPU, once parameters() or train() asked for them
+        self._training = False     # train() was called: forward() is the differentiable one
 
     # ---- reference-compatible surface -------------------------------------------------------------
     def get_model_type(self):
@@ -71,6 +77,8 @@ class ModelBiLSTM(object):
         return spec
 
     def state_dict(self):
+        if self._training:
+            self._take_leaves()
         return OrderedDict((k, v.clone()) for k, v in self._params.items())
 
     def load_state_dict(self, state_dict, strict=True):
@@ -92,18 +100,61 @@ class ModelBiLSTM(object):
         for k in self._params:
             if k in state_dict:
                 self._params[k] = state_dict[k].detach().to(device="cpu", dtype=torch.float32).contiguous().clone()
+        if self._leaves is not None:
+            with torch.no_grad():
+                for k, v in self._leaves.items():
+                    v.copy_(self._params[k])
         self._release()
         return self
 
     def cuda(self, device=None):
         if device is not None:
             self.device = device
-        self._ensure_handle()
+        if self._leaves is not None:
+            for v in self._leaves.values():
+                v.data = v.data.to(torch.device("cuda", self._device_index()))
+        if not self._training:
+            self._ensure_handle()
         return self
 
     def eval(self):
+        """inference: forward() runs the inference kernels, with the values that training left"""
+        if self._training:
+            self._take_leaves()
+            self._release()   # its weights are the ones before training; the next forward repacks
         self._training = False
         return self
+
+    # ---- training -----------------------------------------------------------------------------------
+    def train(self, mode=True):
+        """forward() becomes differentiable in parameters(): dropout as the reference's training has it, initial states drawn
+        by torch.randn (init_state="randn"), zeros, or init_states.  loss: train_ops.cross_entropy; clipping: train_ops.clip_grad_norm_"""
+        if not mode:
+            return self.eval()
+        self.parameters()
+        self._training = True
+        return self
+
+    def named_parameters(self):
+        """(name, leaf tensor on this model's GPU) in state_dict order; they stay the same tensors for the model's life"""
+        if self._leaves is None:
+            dev = torch.device("cuda", self._device_index())
+            self._leaves = OrderedDict((k, v.to(dev).requires_grad_()) for k, v in self._params.items())
+        return list(self._leaves.items())
+
+    def parameters(self):
+        return [v for _, v in self.named_parameters()]
+
+    def zero_grad(self, set_to_none=True):
+        for v in (self._leaves or {}).values():
+            if set_to_none:
+                v.grad = None
+            elif v.grad is not None:
+                v.grad = torch.zeros_like(v.grad)
+
+    def _take_leaves(self):
+        for k, v in self._leaves.items():
+            self._params[k] = v.detach().to(device="cpu", copy=True).contiguous()
 
     def parameters_count(self):
         return sum(v.numel() for v in self._params.values())
@@ -167,6 +218,11 @@ class ModelBiLSTM(object):
         model's GPU; kmer / base_signal_lens may be float32 (reference convention) or uint8/uint16/int32.
         site_keys (init_state="randn" only): int64 / uint64 tensor [B] on the GPU naming each site for the in-kernel
         initial-state generator (dsp_init_state.site_keys); default = self.site_offset + row index."""
+        if self._training:
+            if site_keys is not None:
+                raise ValueError("site_keys name sites for the inference kernels' generator; in training pass init_states")
+            logits, probs = training.forward(self, self._leaves, kmer, base_means, base_stds, base_signal_lens, signals, init_states)
+            return (logits, probs, probs.argmax(1).to(torch.uint8)) if want_labels else (logits, probs)
         self._ensure_handle()
         dev = torch.device("cuda", self._device_index())
         has_seq = self.module != "signal_bilstm"

@@ -3,11 +3,12 @@ around ModelBiLSTM.
 
   embedding        lookup with scaling, gradient by sorted tokens             (nn.Embedding, models.py:186)
   lstm             one layer, one or both directions                          (nn.LSTM, models.py:137-157)
+  linear           a fully connected layer                                    (nn.Linear, models.py:147-161)
   cross_entropy    softmax cross entropy with class weights                   (nn.CrossEntropyLoss)
   clip_grad_norm_  clipping by the norm over many gradients, in place         (nn.utils.clip_grad_norm_)
   clip_grad_norm   the same into other tensors;  grad_norm: the norm alone
 
-The first three are differentiable once by torch's autograd.  Everything runs on the tensors' GPU and its current stream,
+The first four are differentiable once by torch's autograd.  Everything runs on the tensors' GPU and its current stream,
 enqueues kernels only (no copy, no synchronisation; workspaces come from torch's allocator, so a captured call's belong to its
 graph) and gives the same bits for the same inputs and sizes.  There is no CPU path.  ValueError for shapes, types and values;
 RuntimeError for tensors that are not on one GPU."""
@@ -214,6 +215,51 @@ def lstm(x, weights, h0=None, c0=None):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h0, c0, *weights)):
         return _Lstm.apply(x, h0, c0, *weights)
     return _lstm_forward(x, h0, c0, weights, False)[:3]
+
+
+# ---- linear ------------------------------------------------------------------------------------------------------------------
+def _linear_forward(x, weight, bias):
+    outputs, inputs = weight.shape
+    y = x.new_empty((*x.shape[:-1], outputs))
+    _call(x.get_device(), nat.lib().dsp_linear_forward, x.numel() // inputs, inputs, outputs, x.data_ptr(), weight.data_ptr(), _ptr(bias), y.data_ptr())
+    return y
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(x, weight)
+        ctx.has_bias = bias is not None
+        return _linear_forward(x, weight, bias)
+
+    @_differentiable_once
+    def backward(ctx, grad):
+        x, weight = ctx.saved_tensors
+        (outputs, inputs), L = weight.shape, nat.lib()
+        rows, grad = x.numel() // inputs, grad.contiguous()
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw, db = torch.empty_like(weight), weight.new_empty(outputs) if ctx.has_bias else None
+        ws = _workspace(x, L.dsp_linear_workspace(rows, inputs, outputs))
+        _call(x.get_device(), L.dsp_linear_backward, rows, inputs, outputs, x.data_ptr(), weight.data_ptr(), grad.data_ptr(), _ptr(dx), dw.data_ptr(), _ptr(db),
+              ws.data_ptr(), ws.numel())
+        return dx, dw, db
+
+
+def linear(x, weight, bias=None):
+    """x weight^T + bias: [..., outputs] for x [..., inputs], weight [outputs, inputs], bias [outputs]; float32, at most 16,384 inputs
+    and outputs.  (torch's own bias gradient is a sum that clears flags by a memset: captured into a graph, its replays went wrong here.)"""
+    _one_gpu("linear", x, weight, bias)
+    for t in (x, weight, bias):
+        if t is not None and t.dtype != torch.float32:
+            raise ValueError("linear: tensors must be float32, got %s" % t.dtype)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError("linear: x must be [..., inputs] and weight [outputs, inputs], got %s and %s" % (list(x.shape), list(weight.shape)))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError("linear: bias must be [%d], got %s" % (weight.shape[0], list(bias.shape)))
+    x, weight, bias = x.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _Linear.apply(x, weight, bias)
+    return _linear_forward(x, weight, bias)
 
 
 # ---- cross entropy ---------------------------------------------------------------------------------------------------------------

@@ -550,9 +550,9 @@ double dsp_debug_piece_cost(const dsp_model_cfg* cfg, int32_t n_cus, int64_t n_s
  * address there), out[3] = floats of the 4 KiB buffer still 1.0 after 64 out-of-range stores (1,024: dropped). */
 int32_t dsp_debug_range_probe(int32_t device, int32_t out[4]);
 
-/* ---- the operators of a training step (csrc/dsp_embed.hip, dsp_lstm_train.hip, dsp_loss.hip, dsp_clip.hip) ------------------
+/* ---- the operators of a training step (csrc/dsp_embed.hip, dsp_lstm_train.hip, dsp_linear.hip, dsp_loss.hip, dsp_clip.hip)
  * What the reference's `train` (train.py:75-119) computes with torch's own operators around ModelBiLSTM: the embedding
- * lookup (models.py:186), the LSTM layers (models.py:137-157), CrossEntropyLoss with class weights, and
+ * lookup (models.py:186), the LSTM layers (models.py:137-157), the fully connected layers (:147-161), CrossEntropyLoss with class weights, and
  * clip_grad_norm_, each with its gradient.  deepsignal_plant_amd/train_ops.py is the Python side.
  *
  * All pointers but the argument structs, the tables of dsp_clip_grad_norm and the weight tables in dsp_lstm_layer are DEVICE
@@ -607,6 +607,15 @@ int64_t dsp_lstm_workspace(const dsp_lstm_layer* layer);
 int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* layer, const float* x, const float* c0, const float* gates, const float* cells,
                           const float* grad_y, const float* grad_hn, const float* grad_cn, float* dx, float* dh0, float* dc0,
                           const dsp_lstm_grads* grads, void* workspace, int64_t workspace_bytes);
+
+/* A fully connected layer, fp32: y [rows][outputs] = x [rows][inputs] weight^T + bias, weight [outputs][inputs], bias [outputs] or NULL.
+ * Backward: grad_x (NULL: not wanted), grad_weight, grad_bias (NULL: not wanted).  inputs, outputs <= 16,384, rows < 2^30, 0 allowed. */
+int32_t dsp_linear_forward(void* stream, int64_t rows, int64_t inputs, int64_t outputs, const float* x, const float* weight, const float* bias,
+                           float* y);
+int64_t dsp_linear_workspace(int64_t rows, int64_t inputs, int64_t outputs);
+int32_t dsp_linear_backward(void* stream, int64_t rows, int64_t inputs, int64_t outputs, const float* x, const float* weight,
+                            const float* grad_y, float* grad_x, float* grad_weight, float* grad_bias, void* workspace,
+                            int64_t workspace_bytes);
 
 /* Softmax cross entropy of n rows of c logits (rows row_stride values apart) with an optional weight per class, as
  * torch.nn.CrossEntropyLoss: reduction MEAN divides by the sum of the labels' weights (NaN where there are none), NONE

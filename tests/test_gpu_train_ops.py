@@ -634,6 +634,52 @@ def test_lstm_empty_batch_and_views(ops):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+# ---- linear ------------------------------------------------------------------------------------------------------------------------
+def check_linear(ops, shape, inputs, outputs, bias=True, seed=1):
+    """each value is a sum of n products: off by at most n U of the sum of their sizes, and once more by the bias"""
+    g = gen(seed)
+    x, w, b = torch.randn(*shape, inputs, generator=g), torch.randn(outputs, inputs, generator=g), torch.randn(outputs, generator=g) if bias else None
+    gy = torch.randn(*shape, outputs, generator=g)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b) if t is not None]
+    y = ops.linear(*leaves)
+    xd, wd, gd = x.double().reshape(-1, inputs), w.double(), gy.double().reshape(-1, outputs)
+    rows = xd.shape[0]
+    close(y, (xd @ wd.t() + (b.double() if bias else 0)).view(*shape, outputs),
+          (inputs + 1) * U * (xd.abs() @ wd.abs().t() + (b.double().abs() if bias else 0)).view(*shape, outputs) + 1e-30, "y")
+    got = torch.autograd.grad(y, leaves, gy.to(DEV), retain_graph=True)
+    close(got[0], (gd @ wd).view(*shape, inputs), outputs * U * (gd.abs() @ wd.abs()).view(*shape, inputs) + 1e-30, "dx")
+    close(got[1], gd.t() @ xd, (rows + 1) * U * (gd.abs().t() @ xd.abs()) + 1e-30, "dw")
+    if bias:
+        close(got[2], gd.sum(0), (rows + 1) * U * gd.abs().sum(0) + 1e-30, "db")
+    assert all(torch.equal(a, c) for a, c in zip(got, torch.autograd.grad(y, leaves, gy.to(DEV))))
+
+
+@pytest.mark.parametrize("rows", [0, 1, 15, 64, 65, 130, 1000, 6656])
+@pytest.mark.parametrize("inputs,outputs", [(1, 1), (7, 2), (16, 16), (256, 2), (33, 65), (512, 256), (256, 128)])
+def test_linear_sizes(ops, rows, inputs, outputs):
+    check_linear(ops, (rows,), inputs, outputs)
+
+
+def test_linear_shapes_views_and_missing_parts(ops):
+    check_linear(ops, (3, 5, 7), 20, 12)
+    check_linear(ops, (), 20, 12)
+    check_linear(ops, (40,), 20, 12, bias=False)
+    check_linear(ops, (70000,), 24, 36)
+    check_linear(ops, (20000,), 300, 260)
+    x, w, b = (torch.randn(*s, generator=gen(2)).to(DEV) for s in ((90, 48), (32, 48), (32,)))
+    want = ops.linear(x, w, b)
+    off = [torch.empty(t.numel() + 1, device=DEV)[1:].view(t.shape).copy_(t) for t in (x, w, b)]   # not aligned to 16 bytes
+    assert torch.equal(ops.linear(*off), want)
+    assert torch.equal(ops.linear(x.t().contiguous().t(), w.t().contiguous().t(), b), want)
+    only = w.clone().requires_grad_()
+    gw, = torch.autograd.grad(ops.linear(x, only, b).sum(), only)      # x needs no gradient; the gradient of y is one expanded value
+    assert torch.allclose(gw, x.sum(0).expand(32, 48), rtol=2e-5, atol=2e-5)
+    bad = x.clone()
+    bad[7, 3] = math.nan
+    y = ops.linear(bad, w, b)
+    assert torch.isnan(y[7]).all() and int(torch.isnan(y).sum()) == 32
+
+
 @pytest.mark.parametrize("what", ["embedding", "loss", "lstm"])
 def test_gradients_against_differences(ops, what):
     """f(v + e d) - f(v - e d) over 2 e along a random direction d: the difference quotient is off by e^2 of the third derivative, and by

@@ -83,6 +83,26 @@ def test_lstm_refusals_at_the_abi():
     refused(bwd(g, l=layer(missing=("w_hh", 0))), "NULL weight")
 
 
+def test_linear_refusals_at_the_abi():
+    L = nat.lib()
+    size = L.dsp_linear_workspace(8, 4, 2)
+    fwd = lambda m=8, k=4, n=2, x=P, w=P, y=P: L.dsp_linear_forward(None, m, k, n, x, w, None, y)
+    bwd = lambda w=P, gy=P, dw=P, ws=P, size=size: L.dsp_linear_backward(None, 8, 4, 2, P, w, gy, None, dw, None, ws, size)
+    refused(fwd(m=-1), "number of rows")
+    refused(fwd(m=2 ** 30), "number of rows")
+    for bad in (dict(k=0), dict(n=0), dict(k=16385), dict(n=16385)):
+        refused(fwd(**bad), "1 .. 16,384")
+    for k in ("x", "w", "y"):
+        refused(fwd(**{k: None}), "NULL")
+    assert fwd(m=0, x=None, y=None) == 0 and size > 0
+    for k in ("w", "gy", "dw"):
+        refused(bwd(**{k: None}), "NULL")
+    refused(bwd(ws=None), "workspace too small")
+    refused(bwd(size=size - 1), "workspace too small")
+    refused(bwd(ws=P + 16), "256 bytes")
+    refused(L.dsp_linear_workspace(1, 0, 1), "1 .. 16,384")
+
+
 def test_loss_refusals_at_the_abi():
     L = nat.lib()
     size = L.dsp_cross_entropy_workspace(8)
