@@ -268,10 +268,11 @@ class DeviceSiteFrequency(object):
         from . import dist as dsp_dist
         multi = dsp_dist.collective(world)   # several ranks, or a forced one-rank RCCL group (DSP_FORCE_DIST=1)
         if multi:
-            lists = dsp_dist.all_gather_json(list(names), world, dev)   # (chromosome names: json through dist.comm_device)
+            # (chromosome names are bytes of any encoding: through json as latin-1, which keeps every byte)
+            lists = dsp_dist.all_gather_json([nm.decode("latin-1") for nm in names], world, dev)
             glob, ids = [], {}
             for lst in lists:
-                for nm in lst:
+                for nm in (s.encode("latin-1") for s in lst):
                     if nm not in ids:
                         ids[nm] = len(glob)
                         glob.append(nm)
