@@ -470,7 +470,7 @@ __global__ __launch_bounds__(256, 3) void lstm_step_kernel(Shape s, int step, We
             cells[m[j] * H + u] = cell;
             if (step == 0) h_before[m[j] * H + u] = h0 ? h0[at[j]] : 0.0f;
             if (step < T - 1) h_before[(m[j] + after - t) * H + u] = h;
-        } else
+        } else if (step < T - 1)
             cells[(step & 1) * (i64)s.dirs * B * H + at[j]] = cell;
         y[((b * T + t) * s.dirs + d) * H + u] = h;
         if (step == T - 1) {
@@ -580,7 +580,7 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     if (l->batch == 0) return DSP_OK;
     const Shape s = {(int)l->batch, (int)l->steps, (int)l->input, (int)l->hidden, l->directions};
     const bool fused = s.T == 1;   // a single step makes the gates of x itself: nothing is gained by a product of its own
-    if (!x || !y || !hn || !cn || !cells || (!gates && (!fused || save))) return refuse(who, "NULL pointer");
+    if (!x || !y || !hn || !cn || ((!gates || !cells) && (!fused || save))) return refuse(who, "NULL pointer");
     hipStream_t q = (hipStream_t)stream;
     const i64 M = l->batch * l->steps, N = 4ll * s.H, all = s.dirs * M * s.H;
     if (!fused) {

@@ -31,6 +31,10 @@ _LABEL = {torch.uint8: nat.DT_U8, torch.int32: nat.DT_I32, torch.int64: nat.DT_I
 _REDUCE = {"mean": 0, "sum": 1, "none": 2}
 
 
+# lists of tensors go through map(): a loop in Python costs as much as the kernels of a small call
+_dtype, _layout, _shape, _requires_grad = map(attrgetter, ("dtype", "layout", "shape", "requires_grad"))
+
+
 def _one_gpu(who, *tensors):
     """the index of the tensors' GPU (None among them: not given)"""
     dev = -1
@@ -141,20 +145,21 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
 
 # ---- lstm -----------------------------------------------------------------------------------------------------------------------
 def _layer(x, weights):
-    hidden = weights[1].shape[1]
-    l = nat.LstmLayer(x.shape[0], x.shape[1], x.shape[2], hidden, len(weights) // 4)
-    for d in range(l.directions):
-        l.w_ih[d], l.w_hh[d], l.b_ih[d], l.b_hh[d] = (w.data_ptr() for w in weights[4 * d:4 * d + 4])
-    return l
+    p, two = list(map(torch.Tensor.data_ptr, weights)), ctypes.c_void_p * 2
+    if len(p) == 4:
+        p += [None] * 4
+    return nat.LstmLayer(*x.shape, weights[1].shape[1], len(weights) // 4, two(p[0], p[4]), two(p[1], p[5]), two(p[2], p[6]), two(p[3], p[7]))
 
 
 def _lstm_forward(x, h0, c0, weights, save):
     l, new = _layer(x, weights), x.new_empty
     B, T, H, D = l.batch, l.steps, l.hidden, l.directions
-    y, hn, cn, cells = new((B, T, D * H)), new((D, B, H)), new((D, B, H)), new((2, D, B, T if save else 1, H))
-    gates = new((D, B, T, 4 * H)) if save or T > 1 else None
+    y, hn, cn = new((B, T, D * H)), new((D, B, H)), new((D, B, H))
+    gates = cells = None
+    if save or T > 1:
+        gates, cells = new((D, B, T, 4 * H)), new((2, D, B, T if save else 1, H))
     _call(x.get_device(), nat.lib().dsp_lstm_forward, ctypes.byref(l), x.data_ptr(), _ptr(h0), _ptr(c0), y.data_ptr(), hn.data_ptr(), cn.data_ptr(), _ptr(gates),
-          cells.data_ptr(), int(save))
+          _ptr(cells), int(save))
     return y, hn, cn, gates, cells
 
 
@@ -196,23 +201,23 @@ def lstm(x, weights, h0=None, c0=None):
     weights = list(weights)
     if len(weights) not in (4, 8):
         raise ValueError("lstm: expected the 4 weights of one direction or the 8 of two, got %d" % len(weights))
-    _one_gpu("lstm", x, h0, c0, *weights)
-    for t in (x, h0, c0, *weights):
-        if t is not None and t.dtype != torch.float32:
-            raise ValueError("lstm: tensors must be float32, got %s" % t.dtype)
+    given = [t for t in (x, h0, c0, *weights) if t is not None]
+    _one_gpu("lstm", *given)
+    if set(map(_dtype, given)) != {torch.float32}:
+        raise ValueError("lstm: tensors must be float32")
     if x.dim() != 3 or weights[1].dim() != 2:
         raise ValueError("lstm: x must be [batch, steps, input] and weight_hh [4 * hidden, hidden]")
     hidden, dirs = weights[1].shape[1], len(weights) // 4
     want = [(4 * hidden, x.shape[2]), (4 * hidden, hidden), (4 * hidden,), (4 * hidden,)] * dirs
-    for w, shape in zip(weights, want):
-        if tuple(w.shape) != shape:
-            raise ValueError("lstm: a weight has shape %s, expected %s" % (tuple(w.shape), shape))
+    if list(map(_shape, weights)) != want:
+        raise ValueError("lstm: the weights have shapes %s, expected %s" % ([tuple(w.shape) for w in weights], want))
     for name, t in (("h0", h0), ("c0", c0)):
-        if t is not None and tuple(t.shape) != (dirs, x.shape[0], hidden):
+        if t is not None and t.shape != (dirs, x.shape[0], hidden):
             raise ValueError("lstm: %s has shape %s, expected %s" % (name, tuple(t.shape), (dirs, x.shape[0], hidden)))
-    x, h0, c0 = (None if t is None else t.contiguous() for t in (x, h0, c0))
-    weights = [w.contiguous() for w in weights]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, h0, c0, *weights)):
+    if not all(map(torch.Tensor.is_contiguous, given)):
+        x, h0, c0 = (None if t is None else t.contiguous() for t in (x, h0, c0))
+        weights = [w.contiguous() for w in weights]
+    if torch.is_grad_enabled() and any(map(_requires_grad, given)):
         return _Lstm.apply(x, h0, c0, *weights)
     return _lstm_forward(x, h0, c0, weights, False)[:3]
 
@@ -331,9 +336,6 @@ def cross_entropy(logits, labels, weight=None, ignore_index=-100, reduction="mea
 
 
 # ---- the norm of many gradients -----------------------------------------------------------------------------------------------
-_dtype, _layout, _shape = attrgetter("dtype"), attrgetter("layout"), attrgetter("shape")
-
-
 def _is_dense(t):
     """whether the values fill one piece of memory, in whatever order"""
     if t.is_contiguous():
@@ -346,7 +348,6 @@ def _is_dense(t):
     return True
 
 
-# lists of hundreds of tensors go through map(): a loop in Python costs as much as the kernels
 def _check_grads(who, grads):
     """the index of their GPU"""
     for g in grads:
