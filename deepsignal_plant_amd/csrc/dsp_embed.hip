@@ -8,9 +8,10 @@
 // arrival (and serialise where one token is frequent), so both forms below add in an order that the sizes alone decide:
 //   * tables that fit a workgroup's LDS several times over (the model's 16 x 4): every group of lanes keeps a private table
 //     there and walks its own tokens, so the gradient is read once, in order; the tables are joined in a fixed order.
-//   * larger tables: the token numbers are sorted (a stable radix sort, up to 10 bits a pass, carrying the positions), then
-//     groups of lanes walk chunks of the sorted order, each run of equal tokens held in registers.  A run inside a chunk is
-//     written to dW at once; a run that crosses chunks leaves one partial sum per chunk, and a second launch joins those.
+//   * larger tables: the token numbers are sorted (a stable radix sort, up to 10 bits a pass, carrying the positions; few tokens
+//     by counting who comes before whom), then groups of lanes walk chunks of the sorted order, each run of equal tokens held in
+//     registers.  A run inside a chunk is written to dW at once; a run that crosses chunks leaves one partial sum per chunk, and a
+//     second launch joins those.
 // Sums are held in 32 bits and rounded once to the table's type.
 #include "dsp_ops.h"
 
@@ -265,6 +266,43 @@ __global__ __launch_bounds__(256) void sort_move_kernel(i64 n, Keys keys, const 
     }
 }
 
+// Few tokens: every one counts the tokens that come before it (a smaller key, or the same one earlier): one launch in place of three a
+// pass, n^2 comparisons over as many threads as tokens (4,096 of them: 5 us).  The launch's other workgroups clear the gradient.
+constexpr int kRanked = 4096;
+template <class T>
+__global__ __launch_bounds__(256) void sort_ranked_kernel(int n, Keys keys, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, i64 cells, T* __restrict__ dw) {
+    __shared__ __attribute__((aligned(16))) uint32_t k[kRanked];
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const int blocks = (n + 255) >> 8;
+    if ((int)blockIdx.x >= blocks) {
+        const i64 step = (i64)(gridDim.x - blocks) * 256;
+        for (i64 i = (i64)(blockIdx.x - blocks) * 256 + threadIdx.x; i < cells; i += step) dw[i] = T{};
+        return;
+    }
+    const int all = (n + 3) & ~3;
+    for (int i = threadIdx.x; i < all; i += 256) k[i] = i < n ? key_at(keys, i) : 0xffffffffu;   // behind the last: before nothing
+    __syncthreads();
+    const int first = blockIdx.x * 256, i = first + threadIdx.x, last = first + 256 < all ? first + 256 : all;
+    const uint32_t mine = i < n ? k[i] : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < first; j += 4) {
+        const u32x4 x = *(const u32x4*)(k + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += x[e] <= mine;
+    }
+    for (int j = first; j < last; ++j) rank += k[j] < mine || (k[j] == mine && j < i);
+#pragma unroll 4
+    for (int j = last; j < all; j += 4) {
+        const u32x4 x = *(const u32x4*)(k + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += x[e] < mine;
+    }
+    if (i >= n) return;
+    key_out[rank] = mine;
+    pos_out[rank] = (uint32_t)i;
+}
+
 // ---- gradient by sorted tokens ------------------------------------------------------------------------------------------
 template <class T> __global__ __launch_bounds__(256) void embed_zero_kernel(i64 n, T* __restrict__ dw) {
     for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < n; i += (i64)gridDim.x * 256) dw[i] = T{};
@@ -467,20 +505,27 @@ void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, cons
             hipLaunchKernelGGL((embed_grad_small_join_kernel<T>), dim3((unsigned)cdiv(cells, 4)), dim3(256), 0, s, cells, (int)blocks, part, scale, (T*)dw);
         return;
     }
-    const i64 cells = (i64)vocab * dim;
-    hipLaunchKernelGGL((embed_zero_kernel<T>), dim3((unsigned)(cdiv(cells, 256) < 4096 ? cdiv(cells, 256) : 4096)), dim3(256), 0, s, cells, (T*)dw);
-    if (n == 0) return;
+    const i64 cells = (i64)vocab * dim, zero = cdiv(cells, 256) < 4096 ? cdiv(cells, 256) : 4096;
     const Plan p = plan_sorted(n, vocab, dim);
-    uint32_t *count = (uint32_t*)(ws + p.count), *total = (uint32_t*)(ws + p.total);
     const uint32_t *key = nullptr, *pos = nullptr;
-    for (int k = 0; k < p.passes; ++k) {
-        const Keys keys = {tokens, dt, key, vocab, pad};
-        uint32_t *ko = (uint32_t*)(ws + p.key[k & 1]), *po = (uint32_t*)(ws + p.pos[k & 1]);
-        hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, n, keys, k * p.bits, 1 << p.bits, p.tiles, count);
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << p.bits), dim3(256), 0, s, p.tiles, count, total);
-        hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, n, keys, pos, k * p.bits, p.bits, p.tiles, count, total, ko, po);
-        key = ko;
-        pos = po;
+    if (n > 0 && n <= kRanked) {
+        key = (uint32_t*)(ws + p.key[0]);
+        pos = (uint32_t*)(ws + p.pos[0]);
+        hipLaunchKernelGGL((sort_ranked_kernel<T>), dim3((unsigned)(cdiv(n, 256) + zero)), dim3(256), 0, s, (int)n, (Keys{tokens, dt, nullptr, vocab, pad}),
+                           (uint32_t*)(ws + p.key[0]), (uint32_t*)(ws + p.pos[0]), cells, (T*)dw);
+    } else {
+        hipLaunchKernelGGL((embed_zero_kernel<T>), dim3((unsigned)zero), dim3(256), 0, s, cells, (T*)dw);
+        if (n == 0) return;
+        uint32_t *count = (uint32_t*)(ws + p.count), *total = (uint32_t*)(ws + p.total);
+        for (int k = 0; k < p.passes; ++k) {
+            const Keys keys = {tokens, dt, key, vocab, pad};
+            uint32_t *ko = (uint32_t*)(ws + p.key[k & 1]), *po = (uint32_t*)(ws + p.pos[k & 1]);
+            hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, n, keys, k * p.bits, 1 << p.bits, p.tiles, count);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << p.bits), dim3(256), 0, s, p.tiles, count, total);
+            hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, n, keys, pos, k * p.bits, p.bits, p.tiles, count, total, ko, po);
+            key = ko;
+            pos = po;
+        }
     }
     float* part = (float*)(ws + p.part);
     hipLaunchKernelGGL((embed_grad_walk_kernel<T, VEC>), dim3((unsigned)(cdiv(p.chunks, 256 >> ll) * cdiv(vecs, 64))), dim3(256), 0, s, n, p.chunk, vecs,
