@@ -109,9 +109,10 @@ class _Embedding(torch.autograd.Function):
         n, L = tokens.numel(), nat.lib()
         grad = grad.contiguous()
         out = grad.new_empty((rows, dim))
-        ws = _workspace(grad, L.dsp_embedding_workspace(n, rows, dim))
+        size = L.dsp_embedding_workspace(n, rows, dim)
+        ws = _workspace(grad, size) if size else None
         _call(grad.get_device(), L.dsp_embedding_backward, n, tokens.data_ptr(), _TOKEN[tokens.dtype], grad.data_ptr(), rows, dim, _FLOAT[grad.dtype],
-              padding_idx, scale, out.data_ptr(), ws.data_ptr(), ws.numel())
+              padding_idx, scale, out.data_ptr(), _ptr(ws), size)
         return None, out, None, None
 
 

@@ -572,7 +572,7 @@ enum { DSP_DT_I64 = 4 };
 int32_t dsp_embedding_forward(void* stream, int64_t n, const void* tokens, int32_t token_dtype, const void* weight, int64_t vocab,
                               int64_t dim, int32_t dtype, float scale, void* out);
 /* weight_grad[vocab][dim] = scale * sums of grad[n][dim] by token: all rows are written.  Tokens outside the table and, unless it
- * is -1, tokens equal to padding_idx count for nothing.  Sums in 32 bits. */
+ * is -1, tokens equal to padding_idx count for nothing.  Sums in 32 bits.  A workspace of 0 bytes may be NULL. */
 int64_t dsp_embedding_workspace(int64_t n, int64_t vocab, int64_t dim);
 int32_t dsp_embedding_backward(void* stream, int64_t n, const void* tokens, int32_t token_dtype, const void* grad, int64_t vocab,
                                int64_t dim, int32_t dtype, int64_t padding_idx, float scale, void* weight_grad, void* workspace,

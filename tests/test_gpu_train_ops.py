@@ -86,7 +86,7 @@ def test_embedding_rows_of_every_width(ops, dim, dtype):
         check_embedding(ops, tokens_of(n, rows), table(rows, dim, dtype), scale=1.7)
 
 
-@pytest.mark.parametrize("n", [0, 1, 2, 3, 63, 64, 65, 255, 257, 1023, 1024, 1025, 4095, 4096, 4097, 6656, 70001])
+@pytest.mark.parametrize("n", [0, 1, 2, 3, 63, 64, 65, 255, 257, 1023, 1024, 1025, 4095, 4096, 4097, 8192, 8193, 70001])
 @pytest.mark.parametrize("rows", [1, 2, 16, 64, 65, 1000, 1023, 1024, 70000])
 def test_embedding_lengths_and_tables(ops, n, rows):
     check_embedding(ops, tokens_of(n, rows, torch.int32), table(rows, 4))

@@ -31,10 +31,10 @@ def test_embedding_refusals_at_the_abi():
     refused(fwd(out=None), "NULL")
     refused(fwd(out=P + 2), "not aligned")
     assert fwd(n=0, tokens=None, out=None) == 0
-    size = L.dsp_embedding_workspace(8, 16, 4)
-    bwd = lambda pad=-1, g=P, out=P, ws=P, size=size: L.dsp_embedding_backward(None, 8, P, nat.DT_U8, g, 16, 4, nat.FT_F32, pad, 1.0, out, ws, size)
-    assert size > 0
-    refused(bwd(pad=16), "padding_idx")
+    size = L.dsp_embedding_workspace(8, 1600, 4)
+    bwd = lambda pad=-1, g=P, out=P, ws=P, size=size: L.dsp_embedding_backward(None, 8, P, nat.DT_U8, g, 1600, 4, nat.FT_F32, pad, 1.0, out, ws, size)
+    assert size > 0 and L.dsp_embedding_workspace(8, 16, 4) == 0
+    refused(bwd(pad=1600), "padding_idx")
     refused(bwd(pad=-2), "padding_idx")
     refused(bwd(g=None), "NULL")
     refused(bwd(out=None), "NULL")
