@@ -25,7 +25,7 @@ struct Weights { const float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
 
 // gates = W_ih x + b_ih + b_hh, all steps
 template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
-    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<true, true, TILE>()];
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, TILE>()];
     const int M = s.B * s.T, N = 4 * s.H, n_tiles = (N + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int n0 = tile % (n_tiles * s.dirs), d = n0 / n_tiles, at = (n0 - d * n_tiles) * TILE, m0 = tile / (n_tiles * s.dirs) * TILE;
@@ -37,7 +37,7 @@ template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_in
 
 // dx = sum over directions of dz W_ih
 template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_input_grad_kernel(Shape s, const float* __restrict__ dz, Weights w, float* __restrict__ dx) {
-    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<true, false, TILE>()];
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, false, TILE>()];
     const int M = s.B * s.T, K = 4 * s.H, n_tiles = (s.I + TILE - 1) / TILE;
     const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int n0 = tile % n_tiles * TILE, m0 = tile / n_tiles * TILE;
@@ -51,7 +51,7 @@ template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_in
 template <int TILE, bool FAST>
 __global__ __launch_bounds__(256) void lstm_weight_grad_kernel(Shape s, const float* __restrict__ dz, const float* __restrict__ x, const float* __restrict__ h_before,
                                                                int per_part, float* __restrict__ part) {
-    __shared__ __attribute__((aligned16(16))) float lds[2 * half_floats<false, false, TILE>()];
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<false, false, TILE>()];
     const int M = 4 * s.H, K = s.B * s.T, m_tiles = (M + TILE - 1) / TILE, x_tiles = (s.I + TILE - 1) / TILE, n_tiles = x_tiles + (s.H + TILE - 1) / TILE;
     uint32_t tile = tile_of(blockIdx.x, gridDim.x);
     const int nt = tile % n_tiles;
@@ -159,7 +159,7 @@ __device__ __forceinline__ void turn(f32x4& x) {
 template <int N>
 __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights weights, const float* __restrict__ h0, const float* __restrict__ c0, float* gates, float* cells,
                                                             float* h_before, float* __restrict__ y, float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ __attribute__((aligned16(16))) float lds[N * 16 * 64 > 2 * N * 64 ? N * 16 * 64 : 2 * N * 64];
+    __shared__ __attribute__((aligned(16))) float lds[N * 16 * 64 > 2 * N * 64 ? N * 16 * 64 : 2 * N * 64];
     const int B = s.B, T = s.T, H = s.H, d = blockIdx.x % s.dirs, b0 = blockIdx.x / s.dirs * 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, unit = wave * 16 + (lane & 15), part = lane >> 4;
     const bool real = unit < H;
@@ -423,7 +423,7 @@ template <int S, bool WIDE, bool FUSED>
 __global__ __launch_bounds__(256, 3) void lstm_step_kernel(Shape s, int step, Weights w, const float* __restrict__ x, const float* __restrict__ h0,
                                                         const float* __restrict__ c0, float* gates, float* cells, float* h_before, float* y,
                                                         float* __restrict__ hn, float* __restrict__ cn, int save) {
-    __shared__ __attribute__((aligned16(16))) float lds[step_floats<S, 4>()];
+    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 4>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
     const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15);
@@ -496,7 +496,7 @@ template <int S, bool WIDE>
 __global__ __launch_bounds__(256, 3) void lstm_step_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0,
                                                                 const float* __restrict__ gates, const float* __restrict__ cells, const float* __restrict__ gy,
                                                                 const float* __restrict__ ghn, const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
-    __shared__ __attribute__((aligned16(16))) float lds[step_floats<S, 1>()];
+    __shared__ __attribute__((aligned(16))) float lds[step_floats<S, 1>()];
     const Place p = place_of<S>(s);
     const int d = p.d, B = s.B, T = s.T, H = s.H, t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
     const int row = threadIdx.x >> 4, u = p.u0 + (threadIdx.x & 15), uc = u < H ? u : H - 1;
@@ -550,6 +550,7 @@ const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
     if (B < 0 || T < 1 || I < 1 || H < 1) return "sizes must be positive (the batch may be empty)";
     if (I > 16384 || H > 8192) return "at most 16,384 inputs and 8,192 units";
     if (B > (1 << 22) || T > (1 << 22) || B * T >= (1ll << 30)) return "at most 2^22 sequences, 2^22 steps and 2^30 of both";
+    if (B * H >= (1ll << 31)) return "at most 2^31 - 1 values in a state";   // a step's launch: a thread for each, fewer than 2^32
     if (B * T * (H > I ? H : I) >= (1ll << 37)) return "the layer's activations would not fit any device";
     return nullptr;
 }

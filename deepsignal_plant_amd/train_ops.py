@@ -379,7 +379,7 @@ class _Pieces(object):
             end = stop
 
     def check_apart_from(self, who, others):
-        if not self.spans or not others.spans or self.spans[0][0] >= others.spans[-1][1] or others.spans[0][0] >= self.spans[-1][1]:
+        if not self.spans or not others.spans or others.spans[0][0] >= self.spans[-1][1] or self.spans[0][0] >= max(end for _, end in others.spans):
             return
         other = iter(others.spans)
         at = next(other, None)

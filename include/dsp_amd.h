@@ -598,7 +598,7 @@ typedef struct dsp_lstm_grads {   /* of the same shapes; b_ih and b_hh get the s
  * [directions][batch][hidden].  gates: [directions][batch][steps][4 hidden] scratch.  save = 1 keeps what the backward pass needs in
  * gates and in cells [2][directions][batch][steps][hidden] (the cells, and h before each step); save = 0: cells is scratch of
  * [2][directions][batch][hidden].  batch 0 is allowed; steps 1 is the single step of a running sequence (gates and cells may be
- * NULL then, with save = 0).  input <= 16,384, hidden <= 8,192, batch * steps < 2^30. */
+ * NULL then, with save = 0).  input <= 16,384, hidden <= 8,192, batch * steps < 2^30, batch * hidden < 2^31. */
 int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* layer, const float* x, const float* h0, const float* c0, float* y, float* hn,
                          float* cn, float* gates, float* cells, int32_t save);
 /* gradients of x (dx NULL: not wanted), h0 (dh0 NULL: not wanted), c0 (always written) and all weights, from those of y, hn and

@@ -66,6 +66,7 @@ def test_lstm_refusals_at_the_abi():
     refused(fwd(layer(batch=2 ** 15, steps=2 ** 15)), "2^30 of both")
     refused(fwd(layer(missing=("b_hh", 1))), "NULL weight")
     refused(fwd(layer(batch=2 ** 20, steps=2 ** 9, hidden=2 ** 10)), "would not fit")
+    refused(fwd(layer(batch=2 ** 20, steps=1, hidden=2 ** 11)), "2^31 - 1 values in a state")
     refused(fwd(layer(), x=None), "NULL pointer")
     refused(fwd(layer(), y=None), "NULL pointer")
     assert fwd(layer(batch=0), x=None, y=None) == 0
@@ -173,3 +174,14 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="expected a tensor"):
         ops.embedding([1, 2], w)
     assert float(ops.clip_grad_norm_([], 1.0)) == 0.0 and float(ops.clip_grad_norm_([torch.nn.Parameter(w)], 1.0)) == 0.0
+
+
+def test_overlaps_are_found_behind_a_tensor_inside_another():
+    """an output that overlaps a long gradient which a shorter one, also a view of it, comes after"""
+    from deepsignal_plant_amd.train_ops import _Pieces
+    base = torch.zeros(200)
+    ins = _Pieces([base[:100], base[10:20]])
+    with pytest.raises(ValueError, match="overlaps a gradient"):
+        _Pieces([base[50:60]]).check_apart_from("clip_grad_norm", ins)
+    _Pieces([base[100:110]]).check_apart_from("clip_grad_norm", ins)
+    _Pieces([base[100:110]]).check_apart_from("clip_grad_norm", _Pieces([base[110:120]]))
