@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(i64 n, int vecs, int
     typedef Vec<T, VEC> V;
     const int lane = threadIdx.x & ((1 << log_lanes) - 1);
     const i64 groups = 256 >> log_lanes;
-    const i64 row0 = (i64)blockIdx.x * groups * 4 + (threadIdx.x >> log_lanes);
+    const i64 row0 = block_at() * groups * 4 + (threadIdx.x >> log_lanes);
     int t[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(i64 n, int chunk, 
                                                               float scale, const float* __restrict__ part, T* __restrict__ dw) {
     typedef Vec<float, VEC> F;
     __shared__ F sums[256];
-    const i64 c = blockIdx.x, from = c * chunk, to = from + chunk;
+    const i64 c = block_at(), from = c * chunk, to = from + chunk;
     if (to >= n) return;
     const uint32_t run = key[to], last = key[to - 1], start = key[from], before = from > 0 ? key[from - 1] : 0xffffffffu;
     if (run >= (uint32_t)vocab || last != run || (start == run && before == run)) return;   // no run goes on, or it began in an earlier chunk
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(i64 n, int chunk, 
         if (key[mid * chunk] == run) lo = mid + 1;
         else hi = mid;
     }
-    const int lanes = 1 << log_lanes, groups = 256 >> log_lanes, group = threadIdx.x >> log_lanes, v = blockIdx.y * 64 + (threadIdx.x & (lanes - 1));
+    const int lanes = 1 << log_lanes, groups = 256 >> log_lanes, group = threadIdx.x >> log_lanes, v = blockIdx.z * 64 + (threadIdx.x & (lanes - 1));
     const i64 count = lo - (c + 1), per = (count + groups - 1) / groups;   // partial sums behind the first
     F s;
 #pragma unroll
@@ -490,7 +490,7 @@ Plan plan_sorted(i64 n, i64 vocab, i64 dim) {
 template <class T, int VEC>
 void forward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, const void* w, int vocab, float scale, void* out) {
     const int vecs = dim / VEC, ll = log2_lanes(vecs);
-    hipLaunchKernelGGL((embed_forward_kernel<T, VEC>), dim3((unsigned)cdiv(n, 4 * (256 >> ll))), dim3(256), 0, s, n, vecs, ll, tokens, dt,
+    hipLaunchKernelGGL((embed_forward_kernel<T, VEC>), grid_of(cdiv(n, 4 * (256 >> ll))), dim3(256), 0, s, n, vecs, ll, tokens, dt,
                        (const T*)w, vocab, scale, (T*)out);
 }
 
@@ -535,7 +535,9 @@ void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, cons
                        ll, key, pos, (const T*)g, vocab, scale, part, (T*)dw);
     constexpr int JOIN = VEC < 4 ? VEC : 4;   // columns a lane
     const int jv = dim / JOIN;
-    hipLaunchKernelGGL((embed_grad_join_kernel<T, JOIN>), dim3((unsigned)p.chunks, (unsigned)cdiv(jv, 64)), dim3(256), 0, s, n, p.chunk, p.chunks, jv, log2_lanes(jv),
+    dim3 grid = grid_of(p.chunks);
+    grid.z = (unsigned)cdiv(jv, 64);
+    hipLaunchKernelGGL((embed_grad_join_kernel<T, JOIN>), grid, dim3(256), 0, s, n, p.chunk, p.chunks, jv, log2_lanes(jv),
                        key, vocab, scale, part, (T*)dw);
 }
 

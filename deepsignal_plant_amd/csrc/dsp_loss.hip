@@ -31,6 +31,7 @@ struct Loss {   // what every kernel here is given
     int label_dtype, reduction, parts, skip_unit;
     double* weight_part;     // [weight_parts]: sums of labels' weights;  weight_parts 0: den holds their sum, if it is wanted
     int weight_parts;
+    bool wide;               // 16 bytes of a gradient can be written where 16 bytes of logits are read
 };
 
 enum { kMean = DSP_REDUCE_MEAN, kSum = DSP_REDUCE_SUM, kNone = DSP_REDUCE_NONE };
@@ -85,10 +86,11 @@ __device__ __forceinline__ float factor_of(const Loss& p, float w, double den, i
 // sum of the weights of all labels, where rows' gradients are to be written before all rows have been seen: at most kWeightParts
 // sums, which every workgroup of the rows' launch adds for itself
 constexpr int kWeightParts = 64;
-__global__ __launch_bounds__(256) void loss_weights_kernel(Loss p) {
-    __shared__ double scratch[4];
+__global__ __launch_bounds__(1024) void loss_weights_kernel(Loss p) {
+    __shared__ double scratch[16];
     double s = 0;
-    for (i64 r = (i64)blockIdx.x * 256 + threadIdx.x; r < p.n; r += (i64)gridDim.x * 256) s += weight_of(p, label_at(p, r));
+#pragma unroll 4
+    for (i64 r = (i64)blockIdx.x * 1024 + threadIdx.x; r < p.n; r += (i64)gridDim.x * 1024) s += weight_of(p, label_at(p, r));
     s = block_sum(s, scratch);
     if (threadIdx.x == 0) p.weight_part[blockIdx.x] = s;
 }
@@ -97,9 +99,25 @@ __device__ __forceinline__ double weights_of(const Loss& p) {
     if (p.weight_parts == 0) return p.den ? *p.den : 1.0;
     return wave_sum((int)(threadIdx.x & 63) < p.weight_parts ? p.weight_part[threadIdx.x & 63] : 0.0);
 }
+// Many sums are joined by as many workgroups as fill the device, whose own sums another launch joins: one workgroup would need
+// a microsecond for every few thousand
+constexpr int kJoinParts = 256;
+__global__ __launch_bounds__(1024) void loss_join_parts_kernel(Loss p, double2* __restrict__ out) {
+    __shared__ double scratch[16];
+    double a = 0, b = 0;
+#pragma unroll 4
+    for (i64 i = (i64)blockIdx.x * 1024 + threadIdx.x; i < p.parts; i += kJoinParts * 1024) {
+        a += p.part[i].x;
+        b += p.part[i].y;
+    }
+    a = block_sum(a, scratch);
+    b = block_sum(b, scratch);
+    if (threadIdx.x == 0) out[blockIdx.x] = make_double2(a, b);
+}
 __global__ __launch_bounds__(1024) void loss_join_kernel(Loss p) {
     __shared__ double scratch[16];
     double a = 0, b = 0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < p.parts; i += 1024) {
         a += p.part[i].x;
         b += p.part[i].y;
@@ -112,7 +130,8 @@ __global__ __launch_bounds__(1024) void loss_join_kernel(Loss p) {
 }
 
 // ---- few classes: a group of lanes (a power of two, at most 64) per row, E values a lane -----------------------------------
-// ONE: a single workgroup takes all rows, and the sums need no other launch
+// ONE: a single workgroup takes all rows, and the sums need no other launch (512 rows of 2 classes: 7 us in all, the loss, its gradient and what
+// checks the upstream one).  Else labels, logits, what is kept of a row and its loss are all that is moved: 2^24 rows of 2 bf16 in 124 us.
 template <class T, int E, bool BACKWARD, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 256) void loss_few_kernel(Loss p, int log_lanes) {
     __shared__ double scratch[16];
@@ -125,7 +144,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void loss_few_kernel(Loss p, int 
         all = block_sum(all, scratch);
     } else if (p.grad)
         all = weights_of(p);
-    for (i64 r = (i64)blockIdx.x * groups + (threadIdx.x >> log_lanes); r < p.n; r += ONE ? groups : p.n) {
+    for (i64 r = block_at() * groups + (threadIdx.x >> log_lanes); r < p.n; r += ONE ? groups : p.n) {
         const i64 y = label_at(p, r);
         const float w = weight_of(p, y);
         const T* row = (const T*)p.logits + r * p.stride;
@@ -169,23 +188,27 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void loss_few_kernel(Loss p, int 
     if (ONE) {
         if (p.reduction == kMean) *p.den = all;
         *p.loss = (float)(p.reduction == kMean ? num / all : num);
-    } else
-        p.part[blockIdx.x] = make_double2(num, den);
+    } else if (block_at() < p.parts)
+        p.part[block_at()] = make_double2(num, den);
 }
 
-// ---- many classes: a workgroup per row -------------------------------------------------------------------------------------
-// The row is taken as accesses of VEC values at addresses that are multiples of 16 bytes; those at its ends value by value.
-// R > 0: up to R accesses a thread, held in registers; R = 0: any number, read twice.
-template <class T, int VEC> struct RowOf {
+// ---- many classes: lanes or a workgroup per row ----------------------------------------------------------------------------
+// The row is taken as accesses of VEC values at addresses that are multiples of 16 bytes; those at its ends value by value, and so are all
+// stores where the gradient's rows do not begin at the same place within 16 bytes as the logits'.
+template <class T> struct RowOf {
+    static constexpr int VEC = 16 / sizeof(T);
     typedef Vec<T, VEC> V;
     const T* row;
     T* out;
     int shift;   // values between the aligned address before the row and the row
     int c;
+    bool wide;   // stores
+    __device__ __forceinline__ RowOf(const Loss& p, i64 r)
+        : row((const T*)p.logits + r * p.stride), out((T*)p.grad + r * p.c), shift((int)((size_t)row % 16 / sizeof(T))), c((int)p.c), wide(p.wide) {}
     __device__ __forceinline__ int accesses() const { return (c + shift + VEC - 1) / VEC; }
     __device__ __forceinline__ V load(int j) const {
         const int at = j * VEC - shift;
-        if (VEC > 1 && at >= 0 && at + VEC <= c) return *(const V*)(row + at);
+        if (at >= 0 && at + VEC <= c) return *(const V*)(row + at);
         V x;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x.v[e] = at + e >= 0 && at + e < c ? row[at + e] : (T)(-__builtin_inff());
@@ -193,7 +216,7 @@ template <class T, int VEC> struct RowOf {
     }
     __device__ __forceinline__ void store(int j, const V& x) const {
         const int at = j * VEC - shift;
-        if (VEC > 1 && at >= 0 && at + VEC <= c) {
+        if (wide && at >= 0 && at + VEC <= c) {
             *(V*)(out + at) = x;
             return;
         }
@@ -204,21 +227,101 @@ template <class T, int VEC> struct RowOf {
     __device__ __forceinline__ bool inside(int j, int e) const { return j * VEC - shift + e >= 0 && j * VEC - shift + e < c; }
 };
 
-template <class T, int VEC, int R, bool BACKWARD>
+// Rows of up to 512 accesses: a group of lanes (a power of two, at most 64) per row, R accesses a lane in registers; nothing passes through LDS
+// but the workgroup's sums.  Rows come before their labels are known, ignored ones too: what such rows cost is waiting, not bytes.  (65,536 rows
+// of 2,000 bf16: 62 us for the loss = 4.2 TB/s, 149 with the gradient; 1,048,576 of 300: 250 and 520, where a workgroup a row took 1,428 and 2,630.)
+template <class T, int R, bool BACKWARD>
+__global__ __launch_bounds__(256) void loss_group_kernel(Loss p, int log_lanes) {
+    typedef typename RowOf<T>::V V;
+    constexpr int VEC = RowOf<T>::VEC;
+    __shared__ double scratch[4];
+    if (BACKWARD && p.skip_unit && p.reduction != kNone && *p.upstream == 1.0f) return;
+    const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+    const double all = p.grad ? weights_of(p) : 1.0;
+    const i64 r = block_at() * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
+    double num = 0, den = 0;
+    if (r < p.n) {
+        const i64 y = label_at(p, r);
+        const float w = weight_of(p, y);
+        const bool ignored = y == p.ignore;   // nothing to read then
+        const RowOf<T> row(p, r);
+        const int n = row.accesses();
+        V x[R];
+        float m = -__builtin_inff(), z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (lane + (i << log_lanes) < n) x[i] = row.load(lane + (i << log_lanes));
+        if (BACKWARD) {
+            m = p.stat[r].x;
+            z = p.stat[r].y;
+        } else if (!ignored) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (lane + (i << log_lanes) < n)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) m = fmaxf(m, to_f32(x[i].v[e]));
+            for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (lane + (i << log_lanes) < n)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) z += row.inside(lane + (i << log_lanes), e) ? fast_exp(to_f32(x[i].v[e]) - m) : 0.0f;
+            for (int o = lanes >> 1; o; o >>= 1) z += __shfl_xor(z, o);
+        }
+        if (!BACKWARD && lane == 0) {
+            p.stat[r] = make_float2(m, z);
+            const float l = ignored ? 0.0f : w * loss_of(m, z, y >= 0 && y < p.c ? to_f32(row.row[y]) : 0.0f);
+            if (p.reduction == kNone) p.loss[r] = l;
+            num = l;
+            den = w;
+        }
+        if (p.grad) {
+            const float k = factor_of(p, w, all, r), inv = 1.0f / z;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int j = lane + (i << log_lanes);
+                if (j >= n) continue;
+                V g;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    g.v[e] = from_f32<T>(ignored ? 0.0f : k * (fast_exp(to_f32(x[i].v[e]) - m) * inv - (j * VEC - row.shift + e == y ? 1.0f : 0.0f)));
+                row.store(j, g);
+            }
+        }
+    }
+    if (BACKWARD || p.reduction == kNone) return;
+    num = block_sum(num, scratch);
+    den = block_sum(den, scratch);
+    if (threadIdx.x == 0 && block_at() < p.parts) p.part[block_at()] = make_double2(num, den);
+}
+
+// More: a workgroup per row.  R > 0: up to R accesses a thread, held in registers; R = 0: any number, read twice.  4 accesses a thread keep enough
+// under way; more threads than that needs take the place of other rows (65,536 rows of 8,000 bf16 with their gradient: 438 us for 256 threads,
+// 554 for 512), fewer registers than 8 accesses hide more (8,192 of 32,000: 234 us = 4.5 TB/s for 1,024 threads, 263 for 512, 286 for 256).
+template <class T, int R, bool BACKWARD>
 __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
-    typedef Vec<T, VEC> V;
+    typedef typename RowOf<T>::V V;
+    constexpr int VEC = RowOf<T>::VEC;
     __shared__ float scratch[16];
     if (BACKWARD && p.skip_unit && p.reduction != kNone && *p.upstream == 1.0f) return;
-    const i64 r = blockIdx.x;
+    const i64 r = block_at();
+    if (r >= p.n) return;
+    const int threads = blockDim.x;
+    const RowOf<T> row(p, r);
+    const int n = row.accesses();
+    V x[R ? R : 1];
+    auto load = [&]() {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int j = threadIdx.x + i * threads;
+            if (j < n) x[i] = row.load(j);
+        }
+    };
+    // The row is on its way while its label is; where it is long and its time its bytes', rows that are ignored are not read instead
+    const bool early = R && threads <= 512;
+    if (early) load();
     const i64 y = label_at(p, r);
     const float w = weight_of(p, y);
-    const int threads = blockDim.x;
-    RowOf<T, VEC> row;
-    row.row = (const T*)p.logits + r * p.stride;
-    row.out = (T*)p.grad + r * p.c;
-    row.shift = VEC > 1 ? (int)((size_t)row.row % 16 / sizeof(T)) : 0;
-    row.c = (int)p.c;
-    const int n = row.accesses();
     if (y == p.ignore) {   // nothing to read
         if (!BACKWARD && threadIdx.x == 0) {
             p.stat[r] = make_float2(0.0f, 1.0f);
@@ -232,15 +335,8 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
             for (int j = threadIdx.x; j < n; j += threads) row.store(j, none);
         return;
     }
-    V x[R ? R : 1];
     float m = -__builtin_inff(), z = 0.0f;
-    if (R) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int j = threadIdx.x + i * threads;
-            if (j < n) x[i] = row.load(j);
-        }
-    }
+    if (!early) load();
     if (BACKWARD) {
         m = p.stat[r].x;
         z = p.stat[r].y;
@@ -309,9 +405,13 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-constexpr i64 kFew = 256;   // classes up to which a row is a group of lanes' work
+// Classes up to which a lane takes single values, 4 of them; many rows of more classes than 32 are taken in accesses of 16 bytes instead
+constexpr i64 kFew = 256, kFewOfMany = 32;
+// Accesses up to which a row is a group of lanes' (65,536 rows of bf16, loss alone: 112 us for 2,100 classes, 233 by a workgroup each; 65,536 of
+// 4,100: 329 against 180)
+constexpr i64 kGroupMost = 512;
 
-constexpr i64 kOne = 4096;  // lanes' worth of rows up to which one workgroup takes them all: 3 launches less, 4 rows a group at most
+constexpr i64 kOne = 4096;  // lanes' worth of rows up to which one workgroup takes them all: 2 launches less, 4 rows a group at most
 
 int few_lanes(i64 c) {   // 4 values a lane
     int ll = 0;
@@ -320,42 +420,41 @@ int few_lanes(i64 c) {   // 4 values a lane
 }
 bool one_workgroup(i64 n, i64 c) { return c <= kFew && n << few_lanes(c) <= kOne; }
 
-template <class T, bool BACKWARD> i64 launch_rows(hipStream_t s, const Loss& p) {
-    if (p.c <= kFew) {
+// notes in p how many sums there are to join
+template <class T, bool BACKWARD> void launch_rows(hipStream_t s, Loss& p) {
+    const bool one = one_workgroup(p.n, p.c);
+    if (one || p.c <= kFewOfMany) {
         const int ll = few_lanes(p.c);
-        if (!BACKWARD && one_workgroup(p.n, p.c)) {
+        if (!BACKWARD && one) {
             const i64 threads = cdiv(p.n << ll, 64) * 64;
             hipLaunchKernelGGL((loss_few_kernel<T, 4, false, true>), dim3(1), dim3((unsigned)(threads < 1024 ? threads : 1024)), 0, s, p, ll);
-            return 0;
+            return;
         }
-        const i64 blocks = cdiv(p.n, 256 >> ll);
-        hipLaunchKernelGGL((loss_few_kernel<T, 4, BACKWARD, false>), dim3((unsigned)blocks), dim3(256), 0, s, p, ll);
-        return blocks;
+        p.parts = (int)cdiv(p.n, 256 >> ll);
+        hipLaunchKernelGGL((loss_few_kernel<T, 4, BACKWARD, false>), grid_of(p.parts), dim3(256), 0, s, p, ll);
+        return;
     }
-    constexpr int W = 16 / sizeof(T);
-    // wide accesses for the gradient too: its rows must begin at the same place within 16 bytes as the logits' rows
-    const bool wide = !p.grad || ((size_t)p.logits % 16 == (size_t)p.grad % 16 && (p.n == 1 || (p.stride - p.c) * (i64)sizeof(T) % 16 == 0));
-    const i64 vecs = wide ? cdiv(p.c, W) + 1 : p.c;
-    const int threads = vecs <= 256 ? 256 : vecs <= 1024 ? 512 : 1024;
-    const int per = (int)cdiv(vecs, threads);
-#define DSP_ROW(VEC, R) hipLaunchKernelGGL((loss_many_kernel<T, VEC, R, BACKWARD>), dim3((unsigned)p.n), dim3(threads), 0, s, p)
-    if (wide) {
-        if (per <= 1) DSP_ROW(W, 1);
-        else if (per <= 2) DSP_ROW(W, 2);
-        else if (per <= 4) DSP_ROW(W, 4);
-        else if (per <= 8) DSP_ROW(W, 8);
-        else DSP_ROW(W, 0);
-    } else {
-        if (per <= 8) DSP_ROW(1, 8);
-        else DSP_ROW(1, 0);
+    p.wide = (size_t)p.logits % 16 == (size_t)p.grad % 16 && (p.n == 1 || (p.stride - p.c) * (i64)sizeof(T) % 16 == 0);
+    const i64 accesses = cdiv(p.c, 16 / sizeof(T)) + 1;   // at most: whether or not there is a gradient to write, so that the sums are the same
+    if (accesses <= kGroupMost) {
+        int ll = 0;
+        while ((4 << ll) < accesses && ll < 6) ++ll;
+        p.parts = (int)cdiv(p.n, 256 >> ll);
+        if (accesses <= 256) hipLaunchKernelGGL((loss_group_kernel<T, 4, BACKWARD>), grid_of(p.parts), dim3(256), 0, s, p, ll);
+        else hipLaunchKernelGGL((loss_group_kernel<T, 8, BACKWARD>), grid_of(p.parts), dim3(256), 0, s, p, ll);
+        return;
     }
-#undef DSP_ROW
-    return p.n;
+    p.parts = (int)p.n;
+    const int threads = accesses <= 1024 ? 256 : accesses <= 2048 ? 512 : 1024;
+    const int per = (int)cdiv(accesses, threads);
+    if (per <= 4) hipLaunchKernelGGL((loss_many_kernel<T, 4, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    else if (per <= 8) hipLaunchKernelGGL((loss_many_kernel<T, 8, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    else hipLaunchKernelGGL((loss_many_kernel<T, 0, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
 }
-template <bool BACKWARD> i64 launch_typed(hipStream_t s, const Loss& p, int dtype) {
-    if (dtype == DSP_FT_F32) return launch_rows<float, BACKWARD>(s, p);
-    if (dtype == DSP_FT_BF16) return launch_rows<__bf16, BACKWARD>(s, p);
-    return launch_rows<_Float16, BACKWARD>(s, p);
+template <bool BACKWARD> void launch_typed(hipStream_t s, Loss& p, int dtype) {
+    if (dtype == DSP_FT_F32) launch_rows<float, BACKWARD>(s, p);
+    else if (dtype == DSP_FT_BF16) launch_rows<__bf16, BACKWARD>(s, p);
+    else launch_rows<_Float16, BACKWARD>(s, p);
 }
 
 const char* bad_loss(i64 n, i64 c, i64 stride, int dtype, int label_dtype, int reduction) {
@@ -372,7 +471,7 @@ const char* bad_loss(i64 n, i64 c, i64 stride, int dtype, int label_dtype, int r
 
 extern "C" {
 
-int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)(n * sizeof(double2) + kWeightParts * sizeof(double) + 16); }
+int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)((n + kJoinParts) * sizeof(double2) + kWeightParts * sizeof(double)); }
 
 int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride, const void* labels,
                                   int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction, float* loss, float* stat,
@@ -384,13 +483,19 @@ int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void
     if ((reduction != kNone && !loss) || (reduction == kMean && !weight_sum)) return refuse(who, "NULL pointer");
     if ((size_t)workspace & 255) return refuse(who, "the workspace must be aligned to 256 bytes");
     Loss p = {logits, labels, weight, grad, loss, (float2*)stat, weight_sum, (double2*)workspace, nullptr, n, c, row_stride, ignore_index, label_dtype, reduction, 0, 0,
-              (double*)((double2*)workspace + n), 0};
+              (double*)((double2*)workspace + n + kJoinParts), 0};
     hipStream_t s = (hipStream_t)stream;
     if (grad && reduction == kMean && n && !one_workgroup(n, c)) {
-        p.weight_parts = (int)(cdiv(n, 256) < kWeightParts ? cdiv(n, 256) : kWeightParts);
-        hipLaunchKernelGGL(loss_weights_kernel, dim3(p.weight_parts), dim3(256), 0, s, p);
+        p.weight_parts = (int)(cdiv(n, 1024) < kWeightParts ? cdiv(n, 1024) : kWeightParts);
+        hipLaunchKernelGGL(loss_weights_kernel, dim3(p.weight_parts), dim3(1024), 0, s, p);
     }
-    p.parts = n ? (int)launch_typed<false>(s, p, dtype) : 0;
+    if (n) launch_typed<false>(s, p, dtype);
+    if (reduction != kNone && p.parts > kJoinParts * 64) {   // up to 16,384 one workgroup takes no longer than another launch
+        double2* joined = p.part + n;
+        hipLaunchKernelGGL(loss_join_parts_kernel, dim3(kJoinParts), dim3(1024), 0, s, p, joined);
+        p.part = joined;
+        p.parts = kJoinParts;
+    }
     if (reduction != kNone && (n == 0 || !one_workgroup(n, c))) hipLaunchKernelGGL(loss_join_kernel, dim3(1), dim3(1024), 0, s, p);
     return launched(who);
 }

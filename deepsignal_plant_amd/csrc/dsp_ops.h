@@ -51,6 +51,14 @@ inline int launched(const char* who) {
     return DSP_EHIP;
 }
 
+// A launch of any number of workgroups (of at most 1,024 threads): a grid has fewer than 2^32 threads along each of its axes, so many
+// workgroups go along two.  The last row of them may be surplus.
+inline dim3 grid_of(long long blocks) {
+    const long long x = blocks < (1 << 21) ? blocks : 1 << 21;
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ i64 block_at() { return (i64)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline i64 cdiv(i64 a, i64 b) { return (a + b - 1) / b; }
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // largest power of two of at most 16 bytes that divides `bytes` and every address given

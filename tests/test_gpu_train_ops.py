@@ -193,6 +193,24 @@ def test_embedding_offsets_past_32_bits(ops):
     assert float(dw[-1, -1]) == 2.0 and int((dw != 0).sum()) == 1
 
 
+def test_embedding_of_tokens_along_two_axes_of_a_grid(ops):
+    """more workgroups than one axis takes, forward and where the runs are joined; sums of small whole numbers are exact"""
+    n = 2 ** 25 + 7
+    t, w = torch.randint(0, 1000, (n,), device=DEV, dtype=torch.int32), torch.randn(1000, 33, device=DEV).to(BF16)
+    out = ops.embedding(t, w)
+    for part in (slice(0, 4000), slice(n - 4000, n)):
+        assert torch.equal(out[part], w[t[part].long()])
+    del out
+    n = 2 ** 27 + 77
+    t = torch.randint(0, 20000, (n,), device=DEV, dtype=torch.int32)
+    t[-3000:] = 19999
+    w = torch.zeros(20000, 1, device=DEV, requires_grad=True)
+    g = torch.randint(-1, 2, (n, 1), device=DEV).float()
+    dw, = torch.autograd.grad(ops.embedding(t, w), w, g)
+    want = torch.bincount(t[g[:, 0] == 1], minlength=20000) - torch.bincount(t[g[:, 0] == -1], minlength=20000)
+    assert torch.equal(dw[:, 0].long(), want)
+
+
 # ---- cross entropy ----------------------------------------------------------------------------------------------------------------
 def check_loss(ops, logits, labels, weight=None, ignore_index=-100, reduction="mean", upstream=None):
     """logits on the GPU.  Per row: e^(x - m) is off by 2^-22 and |x - m| 2^-23 of itself, a sum of them by at most 64 additions in
@@ -368,6 +386,46 @@ def test_loss_large_values_keep_their_probabilities(ops):
         p = torch.softmax(x.detach().double().cpu(), 1)
         p[torch.arange(8), y.cpu()] -= 1
         assert ((dx.double().cpu() - p).abs() / (p.abs() + 1e-9)).max() < 2.0 ** -15
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c", [20, 32, 33, 63, 64, 129, 200, 256, 1020, 1021, 2040, 2041, 2044, 2045, 4088, 4089, 4096, 4097])
+def test_loss_rows_by_groups_of_lanes(ops, c, dtype):
+    """rows for which one workgroup is too few, classes around each number of lanes and accesses; rows beginning anywhere"""
+    n = 1100 if c < 300 else 9
+    x, y = logits_of(n, c + 3, dtype), labels_of(n, c)
+    y[::7] = -100
+    check_loss(ops, x[:, 3:], y)
+    check_loss(ops, x[:, :c].contiguous(), y, reduction="none", upstream=torch.randn(n, generator=gen(5)))
+
+
+@pytest.mark.parametrize("n, c", [(600001, 20), (2200001, 40), (70001, 700), (17001, 5000)])
+def test_loss_of_many_rows_is_the_sum_of_its_rows(ops, n, c):
+    """more sums than one workgroup joins: they are the rows' losses added in 64 bits, rounded once (and the mean's quotient with them)"""
+    x = torch.randn(n, c, device=DEV, dtype=BF16)
+    y = torch.randint(0, c, (n,), device=DEV)
+    rows = ops.cross_entropy(x, y, reduction="none").double()
+    total = float(rows.cpu().sum())
+    assert abs(float(ops.cross_entropy(x, y, reduction="sum")) - total) <= total * U * 1.001
+    assert abs(float(ops.cross_entropy(x, y)) - total / n) <= total / n * U * 1.001
+    loss = ops.cross_entropy(x.requires_grad_(), y)
+    assert abs(float(loss.detach()) - total / n) <= total / n * U * 1.001
+
+
+@pytest.mark.parametrize("n, c, more", [(2 ** 21 + 3, 4099, 1), (2 ** 23 + 5, 1021, 1), (2 ** 26 + 9, 30, 0)])
+def test_loss_of_rows_along_two_axes_of_a_grid(ops, n, c, more):
+    """more workgroups than one axis takes: the rows at the end are what they are by themselves"""
+    x = torch.randn(1, c + more, device=DEV).to(BF16).expand(n, c + more).contiguous()
+    x[-4000:] = torch.randn(4000, c + more, device=DEV).to(BF16)
+    x = x[:, :c]
+    y = torch.randint(0, c, (n,), device=DEV)
+    x.requires_grad_()
+    loss = ops.cross_entropy(x, y, reduction="none")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    for part in (slice(0, 4000), slice(n - 4000, n)):
+        e = x.detach()[part].requires_grad_()
+        l = ops.cross_entropy(e, y[part], reduction="none")
+        assert torch.equal(l, loss[part]) and torch.equal(torch.autograd.grad(l, e, torch.ones_like(l))[0], dx[part])
 
 
 # ---- the norm of gradients ---------------------------------------------------------------------------------------------------------
