@@ -6,7 +6,7 @@
 //
 // The gradient needs the rows of g by token.  Atomic additions into dW would make the result depend on the order of
 // arrival (and serialise where one token is frequent), so both forms below add in an order that the sizes alone decide:
-//   * tables that fit a workgroup's LDS several times over (the model's 16 x 4): every group of lanes keeps a private table
+//   * small tables of short rows (the model's 16 x 4) fit a workgroup's LDS many times over: every group of lanes keeps a private table
 //     there and walks its own tokens, so the gradient is read once, in order; the tables are joined in a fixed order.
 //   * larger tables: the token numbers are sorted (a stable radix sort, up to 10 bits a pass, carrying the positions; few tokens
 //     by counting who comes before whom), then groups of lanes walk chunks of the sorted order, each run of equal tokens held in
@@ -266,39 +266,42 @@ __global__ __launch_bounds__(256) void sort_move_kernel(i64 n, Keys keys, const 
     }
 }
 
-// Few tokens: every one counts the tokens that come before it (a smaller key, or the same one earlier): one launch in place of three a
-// pass, n^2 comparisons over as many threads as tokens (1,000: 7.8 us with the clearing of 320,000 values, 4,096: 64 us, of which the clearing of 12.8 M values is most).  The launch's other workgroups clear the gradient.
+// Few tokens: every one counts the tokens that come before it (a smaller key, or the same one earlier), one launch in place of three a pass.  A
+// workgroup takes 64 tokens, a wave of it a quarter of what they are compared with.  The launch's other workgroups clear the gradient.
 constexpr int kRanked = 4096;
 template <class T>
 __global__ __launch_bounds__(256) void sort_ranked_kernel(int n, Keys keys, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, i64 cells, T* __restrict__ dw) {
     __shared__ __attribute__((aligned(16))) uint32_t k[kRanked];
+    __shared__ int ranks[4][64];
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const int blocks = (n + 255) >> 8;
+    const int blocks = (n + 63) >> 6;
     if ((int)blockIdx.x >= blocks) {
         const i64 step = (i64)(gridDim.x - blocks) * 256;
         for (i64 i = (i64)(blockIdx.x - blocks) * 256 + threadIdx.x; i < cells; i += step) dw[i] = T{};
         return;
     }
-    const int all = (n + 3) & ~3;
+    const int all = (n + 15) & ~15;
     for (int i = threadIdx.x; i < all; i += 256) k[i] = i < n ? key_at(keys, i) : 0xffffffffu;   // behind the last: before nothing
     __syncthreads();
-    const int first = blockIdx.x * 256, i = first + threadIdx.x, last = first + 256 < all ? first + 256 : all;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * 64, i = first + lane, last = first + 64 < all ? first + 64 : all;
+    const int from = wave * (all / 4), to = from + all / 4;
     const uint32_t mine = i < n ? k[i] : 0;
     int rank = 0;
+    auto count = [&](int lo, int hi, uint32_t below) {   // lo, hi: multiples of 4
 #pragma unroll 4
-    for (int j = 0; j < first; j += 4) {
-        const u32x4 x = *(const u32x4*)(k + j);
+        for (int j = lo; j < hi; j += 4) {
+            const u32x4 x = *(const u32x4*)(k + j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) rank += x[e] <= mine;
-    }
-    for (int j = first; j < last; ++j) rank += k[j] < mine || (k[j] == mine && j < i);
-#pragma unroll 4
-    for (int j = last; j < all; j += 4) {
-        const u32x4 x = *(const u32x4*)(k + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) rank += x[e] < mine;
-    }
-    if (i >= n) return;
+            for (int e = 0; e < 4; ++e) rank += x[e] < below;
+        }
+    };
+    count(from, to < first ? to : first, mine + 1);
+    for (int j = from > first ? from : first; j < (to < last ? to : last); ++j) rank += k[j] < mine + (j < i ? 1u : 0u);
+    count(from > last ? from : last, to, mine);
+    ranks[wave][lane] = rank;
+    __syncthreads();
+    if (wave || i >= n) return;
+    rank = ranks[0][lane] + ranks[1][lane] + ranks[2][lane] + ranks[3][lane];
     key_out[rank] = mine;
     pos_out[rank] = (uint32_t)i;
 }
@@ -442,21 +445,17 @@ constexpr size_t kSmallLds = 64 * 1024;   // two workgroups a CU
 // groups of lanes (a power of two, `most` at first) whose tables fit a workgroup's LDS together
 int groups_that_fit(i64 vocab, i64 dim, int most) {
     while (most > 1 && (size_t)vocab * dim * 4 * most > kSmallLds) most >>= 1;
-    return (size_t)vocab * dim * 4 * most > kSmallLds ? 0 : most;
+    return most;
 }
-// the private tables are the better way where a wave's worth of groups (of 4 values a lane) has one each: 64 rows for dims up to 256
-bool small_table(i64 vocab, i64 dim) {
-    const int wave = 64 >> log2_lanes((int)cdiv(dim, 4));
-    return groups_that_fit(vocab, dim, wave) == wave;
-}
+int few_lanes(i64 dim) { return log2_lanes((int)cdiv(dim, 4)); }
+// Tables of up to 2 KB, of which 32 fit, and rows of up to 16 values, so that many tokens are walked at once.  (2^20 tokens: 64 rows of 8: 54 us,
+// sorted 78; 32 of 16: 59 and 67; but 64 of 16: 91 and 71, 8 of 64: 123 and 90, 64 of 64: 424 and 94)
+bool small_table(i64 vocab, i64 dim) { return dim <= 16 && vocab * dim <= 512; }
 int type_size(int dt) { return dt == DSP_FT_F32 ? 4 : 2; }
-// Few tokens: one workgroup, which needs no second launch and no workspace (6,656 x 16 x 4: 14 us on the GPU in place of 9, 78 in place of
-// 84 us a step of forward and backward, which the host's side bounds).  Else 4 tokens a group at least, the loads that it has under way at once.
+// Few tokens: one workgroup, which needs no second launch and no workspace, where 64 of them are walked at once (6,656 x 16 x 4: 14 us on the GPU in
+// place of 9, 78 in place of 84 us a step of forward and backward, which the host's side bounds; 8,000 of 64 x 8, 32 at once: 91 and 66)
 constexpr i64 kSmallOne = 8192;
-i64 small_blocks(i64 n, int groups) {
-    const i64 b = n <= kSmallOne ? 1 : cdiv(n, (i64)groups * 4);
-    return b > 512 ? 512 : b;
-}
+bool one_workgroup(i64 n, i64 vocab, i64 dim) { return n <= kSmallOne && groups_that_fit(vocab, dim, 256 >> few_lanes(dim)) >= 64; }
 int key_bits(i64 vocab) {   // keys 0 .. vocab
     int b = 1;
     while (((i64)1 << b) <= vocab) ++b;
@@ -498,9 +497,11 @@ template <class T, int VEC>
 void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, const void* g, int vocab, int pad, float scale, void* dw, char* ws) {
     const int vecs = dim / VEC, ll = log2_lanes(vecs);
     if (small_table(vocab, dim)) {
-        // several workgroups: of one wave until there are 512 of them (fewer tables to clear and to join a token), then of 4
-        const int cells = vocab * dim, use = groups_that_fit(vocab, dim, (n <= kSmallOne || n > 512 * 4 * (64 >> ll) ? 256 : 64) >> ll);
-        const i64 blocks = small_blocks(n, use);
+        // several workgroups: of one wave until there are 512 of them (fewer tables to clear and to join a token), then of 4; 4 tokens a group at
+        // least, the loads that it has under way at once
+        const bool one = one_workgroup(n, vocab, dim);
+        const int cells = vocab * dim, use = groups_that_fit(vocab, dim, (one || n > 512 * 4 * (64 >> ll) ? 256 : 64) >> ll);
+        const i64 most = cdiv(n, (i64)use * 4), blocks = one || most < 1 ? 1 : most < 512 ? most : 512;
         float* part = blocks > 1 ? (float*)ws : nullptr;
         hipLaunchKernelGGL((embed_grad_small_kernel<T, VEC>), dim3((unsigned)blocks), dim3(use << ll), (size_t)cells * use * 4, s, n, cdiv(n, blocks), vecs, ll,
                            tokens, dt, (const T*)g, vocab, pad, scale, part, (T*)dw);
@@ -514,7 +515,7 @@ void backward_of(hipStream_t s, i64 n, int dim, const void* tokens, int dt, cons
     if (n > 0 && n <= kRanked) {
         key = (uint32_t*)(ws + p.key[0]);
         pos = (uint32_t*)(ws + p.pos[0]);
-        hipLaunchKernelGGL((sort_ranked_kernel<T>), dim3((unsigned)(cdiv(n, 256) + zero)), dim3(256), 0, s, (int)n, (Keys{tokens, dt, nullptr, vocab, pad}),
+        hipLaunchKernelGGL((sort_ranked_kernel<T>), dim3((unsigned)(cdiv(n, 64) + zero)), dim3(256), 0, s, (int)n, (Keys{tokens, dt, nullptr, vocab, pad}),
                            (uint32_t*)(ws + p.key[0]), (uint32_t*)(ws + p.pos[0]), cells, (T*)dw);
     } else {
         hipLaunchKernelGGL((embed_zero_kernel<T>), dim3((unsigned)zero), dim3(256), 0, s, cells, (T*)dw);
@@ -587,7 +588,7 @@ int32_t dsp_embedding_forward(void* stream, int64_t n, const void* tokens, int32
 
 int64_t dsp_embedding_workspace(int64_t n, int64_t vocab, int64_t dim) {
     if (const char* why = bad_embedding(n, vocab, dim, DSP_DT_U8, DSP_FT_F32)) return refuse("dsp_embedding_workspace", why);
-    if (small_table(vocab, dim)) return n <= kSmallOne ? 0 : (int64_t)align256((size_t)512 * vocab * dim * 4);
+    if (small_table(vocab, dim)) return one_workgroup(n, vocab, dim) ? 0 : (int64_t)align256((size_t)512 * vocab * dim * 4);
     return (int64_t)plan_sorted(n, vocab, dim).bytes;
 }
 

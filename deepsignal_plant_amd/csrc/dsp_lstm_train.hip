@@ -558,6 +558,11 @@ const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
 // workgroup on a CU (4 blocks: 12.3 against 11.3 us at 512 sequences of 256 units, the same at 4,096)
 int step_blocks(const Shape& s) { return cdiv(s.B, 32) * cdiv(s.H, 16) * s.dirs >= 256 ? 2 : 1; }
 
+// Forward, many sequences of more than 64 units: 4 at a time pass a CU in so many turns that the step's larger tiles are faster (128 units, both
+// directions, 13 steps: 1,024 sequences 128 us whole and 121 by steps, 2,048: 231 and 221, 4,096: 455 and 373, 16,384: 1,697 and 1,239).
+// Backward the whole form stays ahead (2,382 and 2,648 us at 16,384), and up to 64 units it does in both (439 and 615).
+bool whole_forward(const Shape& s) { return s.H <= kWholeUnits && (s.H <= 64 || cdiv(s.B, 4) * s.dirs < 2048); }
+
 // the sum over m of the weights' gradients
 Split weight_split(const dsp_lstm_layer* l) { return split_of(l->batch * l->steps, 4 * l->hidden, l->input, l->hidden, l->directions); }
 
@@ -589,7 +594,7 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
         const bool fast = input_wide && s.I % kStep == 0;   // a line's last 16 values are all its own
         DSP_TILES(lstm_inputs_kernel, tile, fast, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
     }
-    if (!fused && s.H <= kWholeUnits) {
+    if (!fused && whole_forward(s)) {
         const dim3 grid((unsigned)(cdiv(s.B, 4) * s.dirs)), block(64 * (unsigned)cdiv(s.H, 16));
         if (s.H > 64) hipLaunchKernelGGL(lstm_whole_kernel<8>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
         else if (s.H > 32) hipLaunchKernelGGL(lstm_whole_kernel<4>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
