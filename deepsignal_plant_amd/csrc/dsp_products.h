@@ -181,6 +181,103 @@ template <int TILE> struct RowSums {
 };
 struct Nothing { template <class V> __device__ __forceinline__ void operator()(const V&) const {} };
 
+// ---- products of few rows or columns ------------------------------------------------------------------------------------------
+// A workgroup of 4 waves makes a tile of 16 S rows by C blocks of 16 columns (a recurrent step forward: the 4 gates of 16 units; backward: 16 units).
+// Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves.  It loads lines of 128 bytes, 8 rows at a
+// time, 32 values of k ahead, and turns them in LDS of its own into what v_mfma_f32_16x16x4 takes (a lane's 4 consecutive k of one
+// row, as above).  Loaded in that form from memory they would cost the L1 an access for each 16 bytes: 16 neighbouring lanes are 16
+// rows (measured: 48 accesses a load, the L1 busy for 80 % of the time, 90 us a step of 4,096 sequences instead of 70).  No wave
+// waits for another until the quarters are joined, in order.  WIDE: rows begin at multiples of 16 bytes and k is one of 4.
+constexpr int kLine = 32;   // values of k at a time
+// where 4 values of a row lie in LDS: the 8 places of a row change with the pair of rows, so that 16 rows read at once fall on all banks
+__device__ __forceinline__ int spread(int row, int k) { return row * kLine + (((k >> 2) ^ (row >> 1)) & 7) * 4; }
+
+// row_a(i): the tile's i-th row;  col_w(i): the tile's i-th column as its offset in bytes from w, below 2^32
+template <int S, int C, bool WIDE, class RowA, class ColW>
+__device__ __forceinline__ void step_product(int K, RowA row_a, const float* w, ColW col_w, float* lds, f32x4 (&acc)[C][S]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = lane >> 3, on = (lane & 7) * 4;
+    const int lines = (K + kLine - 1) / kLine, per = (lines + 3) >> 2, from = wave * per, to = from + per < lines ? from + per : lines;
+    if (from >= to) return;
+    float *la = lds + wave * (S + C) * 16 * kLine, *lw = la + S * 16 * kLine;
+    const float* pa[2 * S];
+    uint32_t pw[2 * C];
+#pragma unroll
+    for (int i = 0; i < 2 * S; ++i) pa[i] = row_a(i * 8 + at) + on;
+#pragma unroll
+    for (int i = 0; i < 2 * C; ++i) pw[i] = col_w(i * 8 + at) + on * 4;
+    f32x4 va[2 * S], vw[2 * C];
+    auto fetch = [&](int line) {
+        const int k = line * kLine;
+        const char* wk = (const char*)(w + k);
+        if (WIDE && k + kLine <= K) {
+#pragma unroll
+            for (int i = 0; i < 2 * S; ++i) va[i] = *(const f32x4*)(pa[i] + k);
+#pragma unroll
+            for (int i = 0; i < 2 * C; ++i) vw[i] = *(const f32x4*)(wk + pw[i]);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = k + on + e < K;
+#pragma unroll
+            for (int i = 0; i < 2 * S; ++i) va[i][e] = in ? pa[i][k + e] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * C; ++i) vw[i][e] = in ? *(const float*)(wk + pw[i] + e * 4) : 0.0f;
+        }
+    };
+    fetch(from);
+    for (int line = from; line < to; ++line) {
+        // one wave's accesses to LDS are carried out in order, and no other wave reads or writes here
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 2 * S; ++i) *(f32x4*)(la + spread(i * 8 + at, on)) = va[i];
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i) *(f32x4*)(lw + spread(i * 8 + at, on)) = vw[i];
+        __builtin_amdgcn_wave_barrier();
+        if (line + 1 < to) fetch(line + 1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f32x4 fa[S], fw[C];
+            const int k = half * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int j = 0; j < S; ++j) fa[j] = *(const f32x4*)(la + spread(j * 16 + (lane & 15), k));
+#pragma unroll
+            for (int c = 0; c < C; ++c) fw[c] = *(const f32x4*)(lw + spread(c * 16 + (lane & 15), k));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j][e], fw[c][e], acc[c][j], 0, 0, 0);
+        }
+    }
+}
+// the sums of the 4 waves: of the values of the tile at the thread's rows (16 apart) and column
+constexpr int kRow = 17;   // floats of a row of 16 in LDS
+template <int S, int C> constexpr int step_floats() {
+    return 4 * (S + C) * 16 * kLine > 4 * C * S * 16 * kRow ? 4 * (S + C) * 16 * kLine : 4 * C * S * 16 * kRow;
+}
+template <int S, int C> __device__ __forceinline__ void step_join(const f32x4 (&acc)[C][S], float* lds, float (&sum)[S][C]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();   // the waves are done with their parts of LDS
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[((wave * C + c) * S * 16 + j * 16 + (lane >> 4) * 4 + r) * kRow + (lane & 15)] = acc[c][j][r];
+    __syncthreads();
+    const int row = threadIdx.x >> 4, unit = threadIdx.x & 15;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            sum[j][c] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[j][c] += lds[((v * C + c) * S * 16 + j * 16 + row) * kRow + unit];
+        }
+}
+
 inline bool aligned16(const void* p) { return (size_t)p % 16 == 0; }
 
 // tiles of 128 x 128 where they fill the device twice, else of 64 x 64

@@ -718,6 +718,14 @@ def test_linear_sizes(ops, rows, inputs, outputs):
     check_linear(ops, (rows,), inputs, outputs)
 
 
+
+@pytest.mark.parametrize("rows, inputs, outputs", [(1, 4096, 700), (16, 1000, 1000), (17, 33, 16), (16385, 40, 16), (5000, 260, 1), (33, 300, 65),
+                                                   (700, 31, 1500), (9000, 128, 130), (4, 12, 2000), (100, 2, 5000)])
+def test_linear_few_rows_or_columns(ops, rows, inputs, outputs):
+    """sums shared by waves, or in parts where the tiles are few; a part's end inside a tile"""
+    check_linear(ops, (rows,), inputs, outputs)
+
+
 def test_linear_shapes_views_and_missing_parts(ops):
     check_linear(ops, (3, 5, 7), 20, 12)
     check_linear(ops, (), 20, 12)
