@@ -298,7 +298,8 @@ __global__ __launch_bounds__(256) void loss_group_kernel(Loss p, int log_lanes) 
 // More: a workgroup per row.  R > 0: up to R accesses a thread, held in registers; R = 0: any number, read twice.  4 accesses a thread keep enough
 // under way; more threads than that needs take the place of other rows (65,536 rows of 8,000 bf16 with their gradient: 438 us for 256 threads,
 // 554 for 512), fewer registers than 8 accesses hide more (8,192 of 32,000: 234 us = 4.5 TB/s for 1,024 threads, 263 for 512, 286 for 256).
-template <class T, int R, bool BACKWARD>
+// EARLY: the row is on its way while its label is; where it is long and its time its bytes', rows that are ignored are not read instead.
+template <class T, int R, bool EARLY, bool BACKWARD>
 __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
     typedef typename RowOf<T>::V V;
     constexpr int VEC = RowOf<T>::VEC;
@@ -317,9 +318,7 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
             if (j < n) x[i] = row.load(j);
         }
     };
-    // The row is on its way while its label is; where it is long and its time its bytes', rows that are ignored are not read instead
-    const bool early = R && threads <= 512;
-    if (early) load();
+    if (EARLY) load();
     const i64 y = label_at(p, r);
     const float w = weight_of(p, y);
     if (y == p.ignore) {   // nothing to read
@@ -336,7 +335,7 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
         return;
     }
     float m = -__builtin_inff(), z = 0.0f;
-    if (!early) load();
+    if (!EARLY) load();
     if (BACKWARD) {
         m = p.stat[r].x;
         z = p.stat[r].y;
@@ -447,9 +446,10 @@ template <class T, bool BACKWARD> void launch_rows(hipStream_t s, Loss& p) {
     p.parts = (int)p.n;
     const int threads = accesses <= 1024 ? 256 : accesses <= 2048 ? 512 : 1024;
     const int per = (int)cdiv(accesses, threads);
-    if (per <= 4) hipLaunchKernelGGL((loss_many_kernel<T, 4, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
-    else if (per <= 8) hipLaunchKernelGGL((loss_many_kernel<T, 8, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
-    else hipLaunchKernelGGL((loss_many_kernel<T, 0, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    if (threads < 1024) hipLaunchKernelGGL((loss_many_kernel<T, 4, true, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    else if (per <= 4) hipLaunchKernelGGL((loss_many_kernel<T, 4, false, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    else if (per <= 8) hipLaunchKernelGGL((loss_many_kernel<T, 8, false, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
+    else hipLaunchKernelGGL((loss_many_kernel<T, 0, false, BACKWARD>), grid_of(p.n), dim3(threads), 0, s, p);
 }
 template <bool BACKWARD> void launch_typed(hipStream_t s, Loss& p, int dtype) {
     if (dtype == DSP_FT_F32) launch_rows<float, BACKWARD>(s, p);
