@@ -58,6 +58,7 @@ class ModelBiLSTM(object):
         self._handle = None
         self._precision = None
         self._leaves = None        # name -> leaf tensor on the GPU, once parameters() or train() asked for them
+        self._taken = None         # the leaves' versions when _params got their values
         self._training = False     # train() was called: forward() is the differentiable one
 
     # ---- reference-compatible surface -------------------------------------------------------------
@@ -77,7 +78,7 @@ class ModelBiLSTM(object):
         return spec
 
     def state_dict(self):
-        if self._training:
+        if self._leaves is not None:
             self._take_leaves()
         return OrderedDict((k, v.clone()) for k, v in self._params.items())
 
@@ -97,6 +98,8 @@ class ModelBiLSTM(object):
                             'current model is {}.'.format(k, tuple(state_dict[k].shape), tuple(v.shape)))
         if errs:
             raise RuntimeError('Error(s) in loading state_dict for ModelBiLSTM:\n\t' + "\n\t".join(errs))
+        if self._leaves is not None:
+            self._take_leaves()   # what state_dict does not hold keeps its trained values
         for k in self._params:
             if k in state_dict:
                 self._params[k] = state_dict[k].detach().to(device="cpu", dtype=torch.float32).contiguous().clone()
@@ -104,6 +107,7 @@ class ModelBiLSTM(object):
             with torch.no_grad():
                 for k, v in self._leaves.items():
                     v.copy_(self._params[k])
+            self._taken = self._versions()
         self._release()
         return self
 
@@ -119,9 +123,8 @@ class ModelBiLSTM(object):
 
     def eval(self):
         """inference: forward() runs the inference kernels, with the values that training left"""
-        if self._training:
+        if self._leaves is not None:
             self._take_leaves()
-            self._release()   # its weights are the ones before training; the next forward repacks
         self._training = False
         return self
 
@@ -140,6 +143,7 @@ class ModelBiLSTM(object):
         if self._leaves is None:
             dev = torch.device("cuda", self._device_index())
             self._leaves = OrderedDict((k, v.to(dev).requires_grad_()) for k, v in self._params.items())
+            self._taken = self._versions()
         return list(self._leaves.items())
 
     def parameters(self):
@@ -152,9 +156,14 @@ class ModelBiLSTM(object):
             elif v.grad is not None:
                 v.grad = torch.zeros_like(v.grad)
 
+    def _versions(self):
+        return [v._version for v in self._leaves.values()]
+
     def _take_leaves(self):
         for k, v in self._leaves.items():
             self._params[k] = v.detach().to(device="cpu", copy=True).contiguous()
+        self._taken = self._versions()
+        self._release()   # its weights are the ones before; the next inference forward repacks
 
     def parameters_count(self):
         return sum(v.numel() for v in self._params.values())
@@ -172,6 +181,8 @@ class ModelBiLSTM(object):
         return int(d)
 
     def _ensure_handle(self):
+        if self._leaves is not None and self._versions() != self._taken:
+            self._take_leaves()   # written to since, by an optimizer or whoever holds them
         if self._handle is not None:
             return
         L = nat.lib()

@@ -27,6 +27,7 @@ from . import _native as nat
 
 _FLOAT = {torch.float32: nat.FT_F32, torch.bfloat16: nat.FT_BF16, torch.float16: nat.FT_F16}
 _TOKEN = {torch.float32: nat.DT_F32, torch.uint8: nat.DT_U8, torch.uint16: nat.DT_U16, torch.int32: nat.DT_I32, torch.int64: nat.DT_I64}
+TOKEN_TYPES = frozenset(_TOKEN)   # of embedding
 _LABEL = {torch.uint8: nat.DT_U8, torch.int32: nat.DT_I32, torch.int64: nat.DT_I64}
 _REDUCE = {"mean": 0, "sum": 1, "none": 2}
 

@@ -51,7 +51,8 @@ def forward(model, p, kmer, base_means, base_stds, base_signal_lens, signals, in
         column = lambda t, name: feature(t, name).reshape(n, L, 1).float()
         x = [column(means, "base_means"), column(base_stds, "base_stds")]
         if model.is_base:
-            x.insert(0, ops.embedding(feature(kmer, "kmer").reshape(n, L), p["embed.weight"]))
+            codes = feature(kmer, "kmer").reshape(n, L)
+            x.insert(0, ops.embedding(codes if codes.dtype in ops.TOKEN_TYPES else codes.float(), p["embed.weight"]))
         if model.is_signallen:
             x.append(column(base_signal_lens, "base_signal_lens"))
         hidden = p["fc_seq.weight"].shape[0]

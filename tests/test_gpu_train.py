@@ -174,6 +174,35 @@ def test_a_training_loop_and_what_the_inference_kernels_get():
     assert all(v.grad is None for v in m.parameters())
 
 
+def test_inference_sees_what_is_written_to_the_parameters():
+    """an optimizer step after eval(), a value written by hand, and a partial state_dict over trained values"""
+    from deepsignal_plant_amd import train_ops as ops
+    cfg, m, w = build(hidden_size=48, num_layers1=2)
+    ins, labels = batch(cfg, 64)
+    dev = [t.to(DEV) for t in ins]
+    m.cuda(0).train()
+    opt = torch.optim.SGD(m.parameters(), lr=0.5)
+    ops.cross_entropy(m(*dev)[0], labels.to(DEV)).backward()
+    m.eval()
+    before = m(*dev)[0].clone()
+    opt.step()
+    after = m(*dev)[0].clone()
+    assert (after - before).abs().max() > 1e-4 and torch.equal(m(*dev)[0], after)
+    leaves = dict(m.named_parameters())
+    with torch.no_grad():
+        leaves["fc2.bias"].add_(1.0)
+    assert (m(*dev)[0] - after - 1.0).abs().max() < 1e-5
+    trained = leaves["fc1.weight"].detach().clone()
+    m.load_state_dict({"fc2.bias": torch.from_numpy(w["fc2.bias"])}, strict=False)
+    assert torch.equal(leaves["fc1.weight"], trained) and torch.equal(m.state_dict()["fc1.weight"], trained.cpu())
+    assert np.array_equal(leaves["fc2.bias"].detach().cpu().numpy(), w["fc2.bias"])
+    kmer, rest = dev[0], dev[1:]
+    m.train()
+    want = m(*dev)[0].detach()
+    for t in (torch.float64, torch.int16, torch.int64, torch.uint8):
+        assert torch.equal(m(kmer.to(t), *rest)[0].detach(), want)
+
+
 def test_a_step_captured_into_a_graph():
     """forward, loss, gradients and clipping of one step as a HIP graph: every replay gives the eager result for the inputs that are in the
     buffers by then, with eager work between the replays; two graphs do not share workspaces"""
