@@ -311,8 +311,7 @@ __global__ __launch_bounds__(256 * M) void lstm_whole_back_kernel(Shape s, Weigh
 
 // ---- the recurrence of more units: a launch per step -------------------------------------------------------------------------
 // By step_product: a workgroup has the 4 gates of 16 units forward, 16 units backward.  A step of both directions, 256 units: 512 sequences 11.4 us
-// either way (47 TFLOP/s: a launch, its ramp and end are half of it), 4,096 sequences 71 us forward and 70 back (60 TFLOP/s, the matrix
-// instructions busy for 47 % of the time: the vector instructions that turn lines in LDS and make the gates share the fp32 datapath).
+// either way (47 TFLOP/s: a launch, its ramp and end are half of it).
 // 16 units fastest, then sequences, then direction, a contiguous range for each die: with two directions it sees one of them, the states
 // of its own sequences and whole lines of their gates
 struct Place { int d, u0, b0; };
@@ -455,6 +454,118 @@ __global__ __launch_bounds__(256, 3) void lstm_step_back_kernel(Shape s, int ste
     }
 }
 
+// ---- the same of many sequences: tiles of 128 or 64 with both operands shared by the workgroup's waves --------------------------
+// Bound by the matrix instructions and, before and behind them, by memory: gates, cells and states, 100 MB a step of 4,096 sequences of 256 units
+// in both directions: 57 us forward (75 TFLOP/s, 1.8 TB/s) and 65 back, by the tiles above 71 and 68.
+// Forward: 128 sequences by the 4 gates of 32 units; a wave has 32 sequences, a lane the 4 gates of one unit of 16 of them, so that the gates
+// meet in registers.  They begin as what the product is added to.
+__global__ __launch_bounds__(256, 2) void lstm_tile_step_kernel(Shape s, int step, Weights w, const float* __restrict__ h0, const float* __restrict__ c0, float* gates, float* cells,
+                                                                float* h_before, float* y, float* __restrict__ hn, float* __restrict__ cn, int save) {
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, 128>()];
+    const int B = s.B, T = s.T, H = s.H, units = (H + 31) >> 5, seqs = (B + 127) >> 7;
+    uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const int u0 = tile % units * 32;
+    tile /= units;
+    const int b0 = tile % seqs * 128, d = tile / seqs;
+    const int t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, u = u0 + (lane & 31), uc = u < H ? u : H - 1;
+    auto sequence = [&](int r) { return b0 + wave * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); };
+    f32x16 acc[1][4];
+    float c[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const i64 b = sequence(r) < B ? sequence(r) : B - 1, at = ((i64)d * B + b) * H + uc, m = ((i64)d * B + b) * T + t;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) acc[0][g][r] = gates[m * 4 * H + g * H + uc];
+        c[r] = step ? save ? cells[(m + before - t) * H + uc] : cells[((step - 1) & 1) * (i64)s.dirs * B * H + at] : c0 ? c0[at] : 0.0f;
+    }
+    auto row_of_w = [&](int row) { return (row >> 5) * H + (row & 31); };   // a unit behind the last is another gate's or zeros, which are not used
+    const Matrix wm = {w.w_hh[d], 4 * H, H};
+    if (step) product<true, true, 128, true>(Matrix{y + ((i64)before * s.dirs + d) * H, B, T * s.dirs * H}, wm, b0, u0, 0, H, lds, acc, Nothing(), row_of_w);
+    else if (h0) product<true, true, 128, true>(Matrix{h0 + (i64)d * B * H, B, H}, wm, b0, u0, 0, H, lds, acc, Nothing(), row_of_w);
+    if (u >= H) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const i64 b = sequence(r);
+        if (b >= B) continue;
+        const i64 at = ((i64)d * B + b) * H + u, m = ((i64)d * B + b) * T + t;
+        const float i = sigmoid(acc[0][0][r]), f = sigmoid(acc[0][1][r]), g = tanh_of(acc[0][2][r]), o = sigmoid(acc[0][3][r]);
+        const float cell = f * c[r] + i * g, h = o * tanh_of(cell);
+        if (save) {
+            float* q = gates + m * 4 * H + u;
+            q[0] = i;
+            q[H] = f;
+            q[2 * H] = g;
+            q[3 * H] = o;
+            cells[m * H + u] = cell;
+            if (step == 0) h_before[m * H + u] = h0 ? h0[at] : 0.0f;
+            if (step < T - 1) h_before[(m + after - t) * H + u] = h;
+        } else if (step < T - 1)
+            cells[(step & 1) * (i64)s.dirs * B * H + at] = cell;
+        y[((b * T + t) * s.dirs + d) * H + u] = h;
+        if (step == T - 1) {
+            hn[at] = h;
+            cn[at] = cell;
+        }
+    }
+}
+
+// Backward: 64 sequences by 64 units, a wave 32 by 32
+__global__ __launch_bounds__(256, 4) void lstm_tile_back_kernel(Shape s, int step, const float* __restrict__ w_hh_t, const float* __restrict__ c0, const float* __restrict__ gates,
+                                                                const float* __restrict__ cells, const float* __restrict__ gy, const float* __restrict__ ghn,
+                                                                const float* __restrict__ gcn, float* dz, float* dc, float* dh0) {
+    __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, 64>()];
+    const int B = s.B, T = s.T, H = s.H, units = (H + 63) >> 6, seqs = (B + 63) >> 6;
+    uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const int u0 = tile % units * 64;
+    tile /= units;
+    const int b0 = tile % seqs * 64, d = tile / seqs;
+    const int t = d ? T - 1 - step : step, before = d ? t + 1 : t - 1, after = d ? t - 1 : t + 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, u = u0 + (wave & 1) * 32 + (lane & 31);
+    auto sequence = [&](int r) { return b0 + (wave >> 1) * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); };
+    f32x16 acc[1][1] = {};
+    if (step < T - 1)
+        product<true, true, 64, true>(Matrix{dz + ((i64)d * B * T + after) * 4 * H, B, T * 4 * H}, Matrix{w_hh_t + (i64)d * H * 4 * H, H, 4 * H}, b0, u0, 0, 4 * H, lds, acc, Nothing());
+    if (u >= H) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {   // 4 rows at a time, the loads of one on their way together
+        float a[4][4], c[4], c_before[4], dct[4], dh[4];
+        i64 at[4], m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const i64 b = sequence(q * 4 + e) < B ? sequence(q * 4 + e) : B - 1;
+            at[e] = ((i64)d * B + b) * H + u;
+            m[e] = ((i64)d * B + b) * T + t;
+            dh[e] = 0.0f;
+            if (step < 0) continue;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) a[e][g] = gates[m[e] * 4 * H + g * H + u];
+            c[e] = cells[m[e] * H + u];
+            c_before[e] = step ? cells[(m[e] + before - t) * H + u] : c0 ? c0[at[e]] : 0.0f;
+            dct[e] = step < T - 1 ? dc[at[e]] : gcn ? gcn[at[e]] : 0.0f;
+            if (step == T - 1 && ghn) dh[e] = ghn[at[e]];
+            if (gy) dh[e] += gy[((b * T + t) * s.dirs + d) * H + u];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (sequence(q * 4 + e) >= B) continue;
+            dh[e] += acc[0][0][q * 4 + e];
+            if (step < 0) {
+                dh0[at[e]] = dh[e];
+                continue;
+            }
+            const float i = a[e][0], f = a[e][1], g = a[e][2], o = a[e][3], tc = tanh_of(c[e]);
+            const float dcell = dct[e] + dh[e] * o * (1.0f - tc * tc);
+            float* z = dz + m[e] * 4 * H + u;
+            z[0] = dcell * g * i * (1.0f - i);
+            z[H] = dcell * c_before[e] * f * (1.0f - f);
+            z[2 * H] = dcell * i * (1.0f - g * g);
+            z[3 * H] = dh[e] * tc * o * (1.0f - o);
+            dc[at[e]] = dcell * f;
+        }
+    }
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------
 const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
     if (dirs != 1 && dirs != 2) return "one direction or two";
@@ -473,6 +584,12 @@ int step_blocks(const Shape& s) { return cdiv(s.B, 32) * cdiv(s.H, 16) * s.dirs 
 // directions, 13 steps: 1,024 sequences 128 us whole and 121 by steps, 2,048: 231 and 221, 4,096: 455 and 373, 16,384: 1,697 and 1,239).
 // Backward the whole form stays ahead (2,382 and 2,648 us at 16,384), and up to 64 units it does in both (439 and 615).
 bool whole_forward(const Shape& s) { return s.H <= kWholeUnits && (s.H <= 64 || cdiv(s.B, 4) * s.dirs < 2048); }
+
+// The forms of many sequences, where the tiles are a workgroup for every CU (forward, whose tiles are larger) or two.  13 steps of both directions, all
+// that belongs to a pass: 2,048 sequences of 1,024 units forward 4,676 -> 3,854 us, back 9,395 -> 7,785; of 256 units, forward 256 tiles, 876 -> 837;
+// 1,024 of 256, 128 tiles, 508 against 581, and 2,048 of 256 back, 256 tiles, 1,635 against 1,740.
+bool tile_forward(const Shape& s) { return s.H % kStep == 0 && cdiv(s.B, 128) * cdiv(s.H, 32) * s.dirs >= 256 && 128ll * s.T * s.dirs * s.H < (1ll << 29); }
+bool tile_backward(const Shape& s) { return s.H % 4 == 0 && cdiv(s.B, 64) * cdiv(s.H, 64) * s.dirs >= 512 && 64ll * s.T * 4 * s.H < (1ll << 29); }
 
 // the sum over m of the weights' gradients
 Split weight_split(const dsp_lstm_layer* l) { return split_of(l->batch * l->steps, 4 * l->hidden, l->input, l->hidden, l->directions); }
@@ -510,6 +627,12 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
         if (s.H > 64) hipLaunchKernelGGL(lstm_whole_kernel<8>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
         else if (s.H > 32) hipLaunchKernelGGL(lstm_whole_kernel<4>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
         else hipLaunchKernelGGL(lstm_whole_kernel<2>, grid, block, 0, q, s, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
+        return launched(who);
+    }
+    if (!fused && tile_forward(s) && hidden_wide) {
+        const dim3 grid((unsigned)(cdiv(s.B, 128) * cdiv(s.H, 32) * s.dirs));
+        for (int step = 0; step < s.T; ++step)
+            hipLaunchKernelGGL(lstm_tile_step_kernel, grid, dim3(256), 0, q, s, step, w, h0, c0, gates, cells, cells + all, y, hn, cn, save);
         return launched(who);
     }
     const int S = step_blocks(s);
@@ -582,10 +705,13 @@ int32_t dsp_lstm_backward(void* stream, const dsp_lstm_layer* l, const float* x,
             hipLaunchKernelGGL(lstm_transpose_kernel, dim3((unsigned)cdiv(s.H, 32), (unsigned)cdiv(4 * s.H, 32), dirs), dim3(256), 0, q, s.H, w, wt);
             const int S = step_blocks(s);
             const bool wide = s.H % 4 == 0;
+            const bool tile = tile_backward(s);
+            const dim3 tiles((unsigned)(cdiv(s.B, 64) * cdiv(s.H, 64) * dirs));
             const dim3 grid((unsigned)(cdiv(s.B, 16 * S) * cdiv(s.H, 16) * dirs));
             for (int step = s.T - 1; step >= (dh0 ? -1 : 0); --step) {
 #define DSP_BACK(S, W) hipLaunchKernelGGL((lstm_step_back_kernel<S, W>), grid, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0)
-                if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
+                if (tile) hipLaunchKernelGGL(lstm_tile_back_kernel, tiles, dim3(256), 0, q, s, step, (const float*)wt, c0, gates, cells, gy, ghn, gcn, dz, dc0, dh0);
+                else if (S == 2) { if (wide) DSP_BACK(2, true); else DSP_BACK(2, false); }
                 else { if (wide) DSP_BACK(1, true); else DSP_BACK(1, false); }
 #undef DSP_BACK
             }

@@ -23,7 +23,9 @@ struct Matrix {   // row-major, `lines` lines of `ld` values
     int lines, ld;
 };
 
-// ALONG_K: a line is a row of the product, k along it.  Else a line is a k, the product's rows along it.
+struct AllLines { __device__ __forceinline__ int operator()(int row) const { return row; } };
+// ALONG_K: a line is a row of the product, k along it.  Else a line is a k, the product's rows along it.  line_of (ALONG_K and FAST): the line
+// that a row of the tile is, from row0
 template <bool ALONG_K, int TILE, bool FAST> struct Stage {
     static constexpr int kStride = ALONG_K ? kStep + 4 : TILE + 4;
     static constexpr int kFloats = ALONG_K ? TILE * kStride : kStep * kStride;
@@ -34,7 +36,7 @@ template <bool ALONG_K, int TILE, bool FAST> struct Stage {
     __amdgpu_buffer_rsrc_t rsrc;
     int lane_at[kLoads];
     uint32_t at, per_step;
-    __device__ __forceinline__ Stage(const Matrix& matrix, int row, int k0, int k1) : m(matrix), row0(row), k_end(k1) {
+    template <class Line = AllLines> __device__ __forceinline__ Stage(const Matrix& matrix, int row, int k0, int k1, Line line_of = {}) : m(matrix), row0(row), k_end(k1) {
         if (!FAST) return;
         const float* base = ALONG_K ? m.p + (i64)row0 * m.ld : m.p + (i64)k0 * m.ld + row0;
         const i64 bytes = ((i64)m.lines * m.ld - (base - m.p)) * 4;
@@ -42,7 +44,7 @@ template <bool ALONG_K, int TILE, bool FAST> struct Stage {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int j = threadIdx.x + i * 256;
-            lane_at[i] = (j / kAcross * m.ld + j % kAcross * 4) * 4;
+            lane_at[i] = (line_of(j / kAcross) * m.ld + j % kAcross * 4) * 4;
         }
         at = ALONG_K ? k0 * 4 : 0;
         per_step = ALONG_K ? kStep * 4 : (uint32_t)m.ld * kStep * 4;
@@ -84,33 +86,34 @@ template <bool A_ALONG_K, bool B_ALONG_K, int TILE> constexpr int half_floats() 
     return Stage<A_ALONG_K, TILE, false>::kFloats + Stage<B_ALONG_K, TILE, false>::kFloats;
 }
 
-// acc[i][j] (block (i, j) of the wave's quarter) += over k in [k0, k1).  f(values of A as they are staged) for every 16 of k
-template <bool A_ALONG_K, bool B_ALONG_K, int TILE, bool FAST, class F>
-__device__ __forceinline__ void product(const Matrix& a, const Matrix& b, int m0, int n0, int k0, int k1, float* lds, f32x16 (&acc)[TILE / 64][TILE / 64], F&& f) {
+// acc[i][j] (block (i, j) of the wave's part of the tile) += over k in [k0, k1).  f(values of A as they are staged) for every 16 of k.  The waves
+// are 2 by 2, or (RM 1, RN 4 of a tile of 128) 4 by 1
+template <bool A_ALONG_K, bool B_ALONG_K, int TILE, bool FAST, int RM, int RN, class F, class Line = AllLines>
+__device__ __forceinline__ void product(const Matrix& a, const Matrix& b, int m0, int n0, int k0, int k1, float* lds, f32x16 (&acc)[RM][RN], F&& f, Line line_of_b = {}) {
     typedef Stage<A_ALONG_K, TILE, FAST> SA;
     typedef Stage<B_ALONG_K, TILE, FAST> SB;
-    constexpr int R = TILE / 64, HALF = SA::kFloats + SB::kFloats;
+    constexpr int HALF = SA::kFloats + SB::kFloats, ACROSS = TILE / 32 / RN;   // waves
+    static_assert(RM * RN * 4 * 32 * 32 == TILE * TILE, "4 waves share the tile");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * (TILE / 2) + (lane & 31), wn = (wave & 1) * (TILE / 2) + (lane & 31), kq = (lane >> 5) * 4;
+    const int wm = wave / ACROSS * (RM * 32) + (lane & 31), wn = wave % ACROSS * (RN * 32) + (lane & 31), kq = (lane >> 5) * 4;
     if (k0 >= k1) return;
     SA sa(a, m0, k0, k1);
-    SB sb(b, n0, k0, k1);
+    SB sb(b, n0, k0, k1, line_of_b);
     auto step = [&](int half, int k) {   // 16 values of k from one half of LDS; the next 16 into the other
         const float *la = lds + half * HALF, *lb = la + SA::kFloats;
 #pragma unroll
         for (int kk = 0; kk < kStep; kk += 8) {
-            f32x4 fa[R], fb[R];
+            f32x4 fa[RM], fb[RN];
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                fa[i] = SA::get(la, wm + i * 32, kk + kq);
-                fb[i] = SB::get(lb, wn + i * 32, kk + kq);
-            }
+            for (int i = 0; i < RM; ++i) fa[i] = SA::get(la, wm + i * 32, kk + kq);
+#pragma unroll
+            for (int j = 0; j < RN; ++j) fb[j] = SB::get(lb, wn + j * 32, kk + kq);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int i = 0; i < R; ++i)
+                for (int i = 0; i < RM; ++i)
 #pragma unroll
-                    for (int j = 0; j < R; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < RN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[i][e], fb[j][e], acc[i][j], 0, 0, 0);
         }
         if (k + kStep < k1) {
             float* next = lds + (half ^ 1) * HALF;

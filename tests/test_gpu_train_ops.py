@@ -633,6 +633,13 @@ def test_lstm_the_models_layers_and_long_sequences(ops, B, T, I, H):
     check_lstm(ops, B, T, I, H)
 
 
+@pytest.mark.parametrize("B,T,I,H,dirs,states", [(1900, 2, 20, 528, 2, True), (1900, 3, 5, 528, 2, False), (3900, 2, 8, 528, 1, True), (4100, 3, 9, 112, 2, True),
+                                                 (4100, 2, 16, 100, 2, True), (8200, 2, 4, 80, 1, False), (16500, 2, 4, 68, 2, True)])
+def test_lstm_many_sequences(ops, B, T, I, H, dirs, states):
+    """the forms of many sequences: tiles that end inside the batch and inside the units, with a last tile of 16 units"""
+    check_lstm(ops, B, T, I, H, dirs=dirs, states=states)
+
+
 def test_lstm_saturated_gates_and_large_inputs(ops):
     """weights six times as large; inputs of 1e6 (an un-normalised read), where every gate is 0 or 1"""
     check_lstm(ops, 33, 13, 16, 32, spread=6.0)
