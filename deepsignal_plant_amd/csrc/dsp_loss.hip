@@ -404,8 +404,9 @@ __global__ __launch_bounds__(1024) void loss_many_kernel(Loss p) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-// Classes up to which a lane takes single values, 4 of them; many rows of more classes than 32 are taken in accesses of 16 bytes instead
-constexpr i64 kFew = 256, kFewOfMany = 32;
+// Classes up to which a lane takes single values, 4 of them; many rows of more classes than one lane has are taken in accesses of 16 bytes
+// instead (2^21 rows, loss alone: 32 bf16 classes 49 us, by single values 128; 8: 26 and 40; 4: 28 and 25)
+constexpr i64 kFew = 256, kFewOfMany = 4;
 // Accesses up to which a row is a group of lanes' (65,536 rows of bf16, loss alone: 112 us for 2,100 classes, 233 by a workgroup each; 65,536 of
 // 4,100: 329 against 180)
 constexpr i64 kGroupMost = 512;
