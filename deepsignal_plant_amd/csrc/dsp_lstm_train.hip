@@ -135,6 +135,9 @@ template <int N> __device__ __forceinline__ f32x4 whole_product(const float* a, 
     }
     return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
+// What has been loaded arrives here, before the stores that follow.  Loads and stores are counted together and in order: a wait behind stores, where the
+// values are used, would be one for the stores as well, a turn to memory in every step.
+template <class T> __device__ __forceinline__ void arrived(T& x) { asm volatile("" : "+v"(x)); }
 // x[i] of 16-lane row r -> x[r] of row i: what a lane has for 4 sequences becomes what it has for 4 gates
 __device__ __forceinline__ void turn(f32x4& x) {
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -199,9 +202,11 @@ __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights wei
     const int t0 = d ? T - 1 : 0, dt = d ? -1 : 1;
 #pragma unroll
     for (int r = 0; r < 4; ++r) next[r] = gates[in[r] + (i64)t0 * 4 * H];
+    float* gates_at = gates + (first + t0) * 4 * H + unit;
+    float *cells_at = cells + (first + t0) * H + unit, *h_at = h_before + (first + t0) * H + unit, *y_at = y + ((b * T + t0) * s.dirs + d) * H + unit;
+    const i64 move = (i64)dt * H;
     for (int step = 0; step < T; ++step) {
         const int t = t0 + step * dt;
-        const i64 m = first + t;
         const f32x4 z0 = next;
         if (step + 1 < T)
 #pragma unroll
@@ -210,21 +215,27 @@ __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights wei
         f32x4 z = whole_product<N>(lds + (step & 1) * N * 64, w) + z0;
         turn(z);
         const float i = sigmoid(z[0]), f = sigmoid(z[1]), g = tanh_of(z[2]), o = sigmoid(z[3]);
-        if (save && step == 0 && store) h_before[m * H + unit] = h;
+        const float h_first = h;
         c = f * c + i * g;
         h = o * tanh_of(c);
         lds[((step & 1) ^ 1) * N * 64 + unit * 4 + part] = real ? h : 0.0f;   // its readers of the step before are behind this step's barrier
-        if (!store) continue;
-        y[((b * T + t) * s.dirs + d) * H + unit] = h;
-        if (save) {
-            float* q = gates + m * 4 * H + unit;
-            q[0] = i;
-            q[H] = f;
-            q[2 * H] = g;
-            q[3 * H] = o;
-            cells[m * H + unit] = c;
-            if (step + 1 < T) h_before[(m + dt) * H + unit] = h;
+        arrived(next);
+        if (store) {
+            *y_at = h;
+            if (save) {
+                if (step == 0) *h_at = h_first;
+                gates_at[0] = i;
+                gates_at[H] = f;
+                gates_at[2 * H] = g;
+                gates_at[3 * H] = o;
+                *cells_at = c;
+                if (step + 1 < T) h_at[move] = h;
+            }
         }
+        y_at += move * s.dirs;
+        gates_at += move * 4;
+        cells_at += move;
+        h_at += move;
     }
     if (store) {
         hn[at] = h;
@@ -255,13 +266,17 @@ __global__ __launch_bounds__(256 * M) void lstm_whole_back_kernel(Shape s, Weigh
     for (int i = threadIdx.x; i < 4 * N * 64; i += 256 * M) dz_lds[i] = 0.0f;   // k beyond the units
     float dc = gcn ? gcn[at] : 0.0f, dh_end = ghn ? ghn[at] : 0.0f;
     float a[4], next[4], c_next = 0.0f, gy_next = 0.0f, c = cells[(first + t0 + (i64)(T - 1) * dt) * H + uc];
-    auto load = [&](int step) {   // gates, the cell before, gradient of y
-        const int t = t0 + step * dt;
-        const i64 m = first + t;
+    const i64 last = first + t0 + (i64)(T - 1) * dt, move = (i64)dt * H;
+    const float *gates_at = gates + last * 4 * H + uc, *cells_at = cells + (last - dt) * H + uc, *gy_at = gy ? gy + ((b * T + t0 + (i64)(T - 1) * dt) * s.dirs + d) * H + uc : nullptr;
+    float* out = dz + last * 4 * H + unit;
+    auto load = [&](int step) {   // gates, the cell before, gradient of y; from the last step down, one at a time
 #pragma unroll
-        for (int g = 0; g < 4; ++g) next[g] = gates[m * 4 * H + g * H + uc];
-        c_next = step ? cells[(m - dt) * H + uc] : c0 ? c0[at] : 0.0f;
-        gy_next = gy ? gy[((b * T + t) * s.dirs + d) * H + uc] : 0.0f;
+        for (int g = 0; g < 4; ++g) next[g] = gates_at[g * H];
+        c_next = step ? *cells_at : c0 ? c0[at] : 0.0f;
+        gy_next = gy ? *gy_at : 0.0f;
+        gates_at -= move * 4;
+        cells_at -= move;
+        if (gy) gy_at -= move * s.dirs;
     };
     load(T - 1);
     for (int step = T - 1; step >= 0; --step) {
@@ -287,13 +302,17 @@ __global__ __launch_bounds__(256 * M) void lstm_whole_back_kernel(Shape s, Weigh
         q[3] = dh * tc * a[3] * (1.0f - a[3]);
         dc = dcell * a[1];
         c = c_before;
-        if (!real) continue;
-        float* out = dz + (first + t0 + (i64)step * dt) * 4 * H + unit;
+        if (real)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            dz_lds[(g * N * 16 + unit) * 4 + seq] = q[g];
-            if (store) out[g * H] = q[g];
-        }
+            for (int g = 0; g < 4; ++g) dz_lds[(g * N * 16 + unit) * 4 + seq] = q[g];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) arrived(next[g]);
+        arrived(c_next);
+        arrived(gy_next);
+        if (store)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) out[g * H] = q[g];
+        out -= move * 4;
     }
     if (dh0) {
         __syncthreads();
