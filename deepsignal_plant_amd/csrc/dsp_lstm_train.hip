@@ -113,8 +113,8 @@ __device__ __forceinline__ float tanh_of(float x) {
 // sequences by 64 columns of one k, the whole of its work useful where the 16 rows of the larger ones would be mostly padding: its
 // 16 blocks all take the same 4 x 1 of A (broadcast from block `k mod 16`, so one register of A serves 16 k) and 4 columns of W
 // each.  What bounds it is the matrix instructions' time (2,048 cycles a step at 128 units) and, behind them, one turn through LDS
-// and the gates: 32 sequences of 128 units, 256 steps, both directions: 425 us forward and 414 back, 1.65 a step, of which the matrix
-// instructions are 0.85.  A launch per step (below) costs 4.5 us instead, at any size: 1.15 ms.
+// and the gates: 32 sequences of 128 units, 256 steps, both directions: 390 us forward and 372 back, 1.5 a step, of which the matrix
+// instructions are 0.85 and the gates 0.16.  A launch per step (below) costs 4.5 us instead, at any size: 1.15 ms.
 //
 // N: 16s of units that the registers are for (8, 4 or 2); units beyond H have weights of zero.
 constexpr int kWholeUnits = 128;
@@ -205,21 +205,10 @@ __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights wei
     float* gates_at = gates + (first + t0) * 4 * H + unit;
     float *cells_at = cells + (first + t0) * H + unit, *h_at = h_before + (first + t0) * H + unit, *y_at = y + ((b * T + t0) * s.dirs + d) * H + unit;
     const i64 move = (i64)dt * H;
-    for (int step = 0; step < T; ++step) {
-        const int t = t0 + step * dt;
-        const f32x4 z0 = next;
-        if (step + 1 < T)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) next[r] = gates[in[r] + (i64)(t + dt) * 4 * H];
-        __syncthreads();   // h of this step is there
-        f32x4 z = whole_product<N>(lds + (step & 1) * N * 64, w) + z0;
-        turn(z);
-        const float i = sigmoid(z[0]), f = sigmoid(z[1]), g = tanh_of(z[2]), o = sigmoid(z[3]);
-        const float h_first = h;
-        c = f * c + i * g;
-        h = o * tanh_of(c);
-        lds[((step & 1) ^ 1) * N * 64 + unit * 4 + part] = real ? h : 0.0f;   // its readers of the step before are behind this step's barrier
-        arrived(next);
+    // A step's values are written while the next one's product is computed, where registers are left for them (389 us in place of 400)
+    constexpr bool LATE = N == 8;
+    float i, f, g, o, h_first = h;
+    auto put = [&](int step) {   // what a step has computed; one at a time
         if (store) {
             *y_at = h;
             if (save) {
@@ -236,7 +225,28 @@ __global__ __launch_bounds__(64 * N) void lstm_whole_kernel(Shape s, Weights wei
         gates_at += move * 4;
         cells_at += move;
         h_at += move;
+    };
+    for (int step = 0; step < T; ++step) {
+        const int t = t0 + step * dt;
+        const f32x4 z0 = next;
+        if (step + 1 < T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) next[r] = gates[in[r] + (i64)(t + dt) * 4 * H];
+        __syncthreads();   // h of this step is there
+        if (LATE && step) put(step - 1);
+        f32x4 z = whole_product<N>(lds + (step & 1) * N * 64, w) + z0;
+        turn(z);
+        i = sigmoid(z[0]);
+        f = sigmoid(z[1]);
+        g = tanh_of(z[2]);
+        o = sigmoid(z[3]);
+        c = f * c + i * g;
+        h = o * tanh_of(c);
+        lds[((step & 1) ^ 1) * N * 64 + unit * 4 + part] = real ? h : 0.0f;   // its readers of the step before are behind this step's barrier
+        arrived(next);
+        if (!LATE) put(step);
     }
+    if (LATE) put(T - 1);
     if (store) {
         hn[at] = h;
         cn[at] = c;
