@@ -58,7 +58,8 @@ class ModelBiLSTM(object):
         self._handle = None
         self._precision = None
         self._leaves = None        # name -> leaf tensor on the GPU, once parameters() or train() asked for them
-        self._taken = None         # the leaves' versions when _params got their values
+        self._taken = None         # the leaves' values on the GPU, as bits, when _params got them
+        self._seen = None          # their addresses and versions then
         self._training = False     # train() was called: forward() is the differentiable one
 
     # ---- reference-compatible surface -------------------------------------------------------------
@@ -107,7 +108,7 @@ class ModelBiLSTM(object):
             with torch.no_grad():
                 for k, v in self._leaves.items():
                     v.copy_(self._params[k])
-            self._taken = self._versions()
+            self._taken, self._seen = self._leaf_bits(), self._leaf_marks()
         self._release()
         return self
 
@@ -143,7 +144,7 @@ class ModelBiLSTM(object):
         if self._leaves is None:
             dev = torch.device("cuda", self._device_index())
             self._leaves = OrderedDict((k, v.to(dev).requires_grad_()) for k, v in self._params.items())
-            self._taken = self._versions()
+            self._taken, self._seen = self._leaf_bits(), self._leaf_marks()
         return list(self._leaves.items())
 
     def parameters(self):
@@ -156,13 +157,28 @@ class ModelBiLSTM(object):
             elif v.grad is not None:
                 v.grad = torch.zeros_like(v.grad)
 
-    def _versions(self):
-        return [v._version for v in self._leaves.values()]
+    def _leaf_marks(self):
+        return [(v.data_ptr(), v._version) for v in self._leaves.values()]
+
+    def _leaf_bits(self):
+        """all leaves' values as one tensor of their bits on this model's GPU"""
+        dev = torch.device("cuda", self._device_index())
+        for k, v in self._leaves.items():
+            if v.shape != self._params[k].shape:
+                raise RuntimeError("parameter %s has shape %s, the model's is %s" % (k, tuple(v.shape), tuple(self._params[k].shape)))
+        return torch.cat([v.detach().to(dev, torch.float32).reshape(-1) for v in self._leaves.values()]).view(torch.int32)
 
     def _take_leaves(self):
-        for k, v in self._leaves.items():
-            self._params[k] = v.detach().to(device="cpu", copy=True).contiguous()
-        self._taken = self._versions()
+        """_params are the leaves' values.  The values themselves are compared: a write through .data, an optimizer's fused step and
+        the replay of a captured one leave no mark on the tensors"""
+        bits = self._leaf_bits()
+        self._seen = self._leaf_marks()
+        if bits.device == self._taken.device and torch.equal(bits, self._taken):
+            return
+        values = bits.cpu().view(torch.float32).split([v.numel() for v in self._params.values()])
+        for (k, v), x in zip(self._params.items(), values):
+            self._params[k] = x.reshape(v.shape).clone()
+        self._taken = bits
         self._release()   # its weights are the ones before; the next inference forward repacks
 
     def parameters_count(self):
@@ -181,8 +197,11 @@ class ModelBiLSTM(object):
         return int(d)
 
     def _ensure_handle(self):
-        if self._leaves is not None and self._versions() != self._taken:
-            self._take_leaves()   # written to since, by an optimizer or whoever holds them
+        if self._leaves is not None:   # whoever holds them may have written to them since
+            if not torch.cuda.is_current_stream_capturing():
+                self._take_leaves()
+            elif self._leaf_marks() != self._seen:   # nothing can be read back here: a captured pass has the weights of the last call before it
+                raise RuntimeError("the parameters were written to since the last inference call: make one, or call eval(), before capturing")
         if self._handle is not None:
             return
         L = nat.lib()

@@ -203,6 +203,58 @@ def test_inference_sees_what_is_written_to_the_parameters():
         assert torch.equal(m(kmer.to(t), *rest)[0].detach(), want)
 
 
+def test_inference_sees_writes_that_leave_no_mark_on_the_parameters():
+    """after eval(): values copied through .data, another tensor put there, a vector of parameters, a fused optimizer's step, the
+    replay of a captured step: none moves a tensor's version, and the next inference call computes with what they wrote"""
+    cfg, m, _ = build(hidden_size=48, num_layers1=1)
+    ins, _ = batch(cfg, 64)
+    dev = [t.to(DEV) for t in ins]
+    m.cuda(0).train()
+    params = m.parameters()
+    for p in params:
+        p.grad = torch.full_like(p, 0.01)
+    m.eval()
+
+    def served(what):
+        _, other, _ = build(hidden_size=48, num_layers1=1)
+        other.load_state_dict({k: v.detach().cpu() for k, v in m.named_parameters()})
+        want = other.cuda(0).eval()(*dev)[0]
+        got = m(*dev)[0].clone()
+        assert torch.equal(got, want), what
+        assert all(torch.equal(v, p.detach().cpu()) for v, p in zip(m.state_dict().values(), params)), what
+        return got
+    before = served("nothing written")
+
+    def moved(what):
+        nonlocal before
+        now = served(what)
+        assert not torch.equal(now, before), what
+        before = now
+    with torch.no_grad():
+        for p in params:
+            p.data.copy_(p * 1.01)
+    moved(".data.copy_")
+    params[-1].data = params[-1].data + 0.5
+    moved(".data =")
+    vector = torch.nn.utils.parameters_to_vector(params).detach() * 0.99
+    torch.nn.utils.vector_to_parameters(vector, params)
+    moved("vector_to_parameters")
+    torch.optim.Adam(params, lr=1e-3, fused=True).step()
+    moved("a fused optimizer's step")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        torch._foreach_add_(params, 0.0)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g), torch.no_grad():
+        torch._foreach_add_(params, [p.grad for p in params])
+    served("a step captured, not run")
+    for _ in range(3):
+        g.replay()
+        moved("a replayed step")
+
+
 def test_a_step_captured_into_a_graph():
     """forward, loss, gradients and clipping of one step as a HIP graph: every replay gives the eager result for the inputs that are in the
     buffers by then, with eager work between the replays; two graphs do not share workspaces"""
