@@ -56,6 +56,8 @@ class ModelBiLSTM(object):
         # parameters start as zeros; real values come from load_state_dict (call_modifications.py:219-223)
         self._params = OrderedDict((k, torch.zeros(shp, dtype=torch.float32)) for k, shp in self._spec)
         self._handle = None
+        self._captured = False     # the handle's memory is part of a captured graph
+        self._retired = []         # handles of which that is so and whose weights are no longer the model's
         self._precision = None
         self._leaves = None        # name -> leaf tensor on the GPU, once parameters() or train() asked for them
         self._taken = None         # the leaves' values on the GPU, as bits, when _params got them
@@ -227,13 +229,17 @@ class ModelBiLSTM(object):
         return self
 
     def _release(self):
-        if self._handle is not None:
+        if self._captured:   # a graph that is replayed again reads its weights and workspace: they live as long as the model
+            self._retired.append(self._handle)
+        elif self._handle is not None:
             nat.lib().dsp_model_destroy(self._handle)
-            self._handle = None
+        self._handle, self._captured = None, False
 
     def __del__(self):
         try:
             self._release()
+            for h in self._retired:
+                nat.lib().dsp_model_destroy(h)
         except Exception:
             pass
 
@@ -309,6 +315,8 @@ class ModelBiLSTM(object):
         probs = torch.empty((n, self.num_classes), dtype=torch.float32, device=dev)
         labels = torch.empty((n,), dtype=torch.uint8, device=dev) if want_labels else None
         stream = torch.cuda.current_stream(dev).cuda_stream
+        with torch.cuda.device(dev):
+            self._captured = self._captured or torch.cuda.is_current_stream_capturing()
 
         def p(t):
             return ctypes.c_void_p(t.data_ptr()) if t is not None else None

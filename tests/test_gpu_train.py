@@ -255,6 +255,48 @@ def test_inference_sees_writes_that_leave_no_mark_on_the_parameters():
         moved("a replayed step")
 
 
+def test_a_captured_inference_pass_outlives_the_weights_it_was_captured_with():
+    """the parameters move on after the capture: eager calls serve them, the replayed pass still has its own weights and workspace, with
+    memory taken and given back in between"""
+    cfg, m, _ = build(hidden_size=48, num_layers1=1)
+    n = 200
+    ins, _ = batch(cfg, n)
+    dev = [t.to(DEV) for t in ins]
+    m.cuda(0).train().eval()
+    m.reserve(n)
+    want = [m(*dev)[0].clone()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m(*dev)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m(*dev)[0]
+        graphs.append((g, out))
+        with torch.no_grad():
+            for p in m.parameters():
+                p.mul_(1.05)
+        with pytest.raises(RuntimeError, match="before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                m(*dev)
+        m.reserve(n)
+        want.append(m(*dev)[0].clone())
+        assert not torch.equal(want[-1], want[-2])
+        m.state_dict()
+        assert torch.equal(m(*dev)[0], want[-1])
+    for _ in range(3):
+        junk = [torch.full((1 << 20,), float("nan"), device=DEV) for _ in range(8)]
+        for (g, out), w in zip(graphs, want):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
+        del junk
+        torch.cuda.empty_cache()
+
+
 def test_a_step_captured_into_a_graph():
     """forward, loss, gradients and clipping of one step as a HIP graph: every replay gives the eager result for the inputs that are in the
     buffers by then, with eager work between the replays; two graphs do not share workspaces"""
