@@ -11,7 +11,7 @@ around ModelBiLSTM.
 The first four are differentiable once by torch's autograd.  Everything runs on the tensors' GPU and its current stream,
 enqueues kernels only (no copy, no synchronisation; workspaces come from torch's allocator, so a captured call's belong to its
 graph) and gives the same bits for the same inputs and sizes.  There is no CPU path.  ValueError for shapes, types and values;
-RuntimeError for tensors that are not on one GPU."""
+RuntimeError for tensors that are not on one GPU, that carry a forward-mode derivative, and inside torch.jit.trace."""
 from __future__ import annotations
 
 import ctypes
@@ -20,6 +20,7 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -36,8 +37,23 @@ _REDUCE = {"mean": 0, "sum": 1, "none": 2}
 _dtype, _layout, _shape, _requires_grad = map(attrgetter, ("dtype", "layout", "shape", "requires_grad"))
 
 
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)   # the public call tests for scripts first, 0.3 us
+
+
+def _refuse_unseen(who, tensors):
+    """What would see an operator's output and not the operator: a trace records the empty output, and a dual tensor's derivative, which
+    requires_grad says nothing of, would be left out, as if it were zero"""
+    if _is_tracing():
+        raise RuntimeError("%s: torch.jit.trace cannot record the library's operators" % who)
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # inside a dual level
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s: no forward-mode derivative is computed" % who)
+
+
 def _one_gpu(who, *tensors):
     """the index of the tensors' GPU (None among them: not given)"""
+    _refuse_unseen(who, tensors)
     dev = -1
     for t in tensors:
         if t is None:
@@ -352,6 +368,7 @@ def _is_dense(t):
 
 def _check_grads(who, grads):
     """the index of their GPU"""
+    _refuse_unseen(who, grads)
     for g in grads:
         if not isinstance(g, torch.Tensor):
             raise ValueError("%s: gradients must be dense tensors" % who)
@@ -429,8 +446,12 @@ def clip_grad_norm(grads, max_norm, out=None):
     max_norm = _max_norm(who, max_norm)
     if not grads:
         raise ValueError("clip_grad_norm: no tensors")
+    if out is not None:
+        out = list(out)
+        _refuse_unseen(who, out)
     dev = _check_grads(who, grads)
-    out = [g.new_empty(g.shape) for g in grads] if out is None else list(out)
+    if out is None:
+        out = [g.new_empty(g.shape) for g in grads]
     if len(out) != len(grads):
         raise ValueError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
     for o in out:

@@ -185,3 +185,41 @@ def test_overlaps_are_found_behind_a_tensor_inside_another():
         _Pieces([base[50:60]]).check_apart_from("clip_grad_norm", ins)
     _Pieces([base[100:110]]).check_apart_from("clip_grad_norm", ins)
     _Pieces([base[100:110]]).check_apart_from("clip_grad_norm", _Pieces([base[110:120]]))
+
+
+def _calls():
+    """name -> (a call of an operator, the tensors of it that can carry a derivative)"""
+    w, x = torch.zeros(16, 4), torch.zeros(3, 4)
+    lstm = [torch.zeros(1, 2, 4), torch.zeros(8, 4), torch.zeros(8, 2), torch.zeros(8), torch.zeros(8), torch.zeros(1, 1, 2), torch.zeros(1, 1, 2)]
+    return {"embedding": (lambda w: ops.embedding(torch.zeros(4, dtype=torch.int64), w), [w]),
+            "lstm": (lambda *t: ops.lstm(t[0], t[1:5], *t[5:]), lstm),
+            "linear": (ops.linear, [x, w, torch.zeros(16)]),
+            "cross_entropy": (lambda x, w: ops.cross_entropy(x, torch.zeros(3, dtype=torch.int64), weight=w), [x, torch.ones(4)]),
+            "grad_norm": (lambda *g: ops.grad_norm(g), [x, w]),
+            "clip_grad_norm": (lambda a, b, c: ops.clip_grad_norm([a, b], 1.0, out=[c, b]), [x, w, torch.zeros(3, 4)])}
+
+
+@pytest.mark.parametrize("name", sorted(_calls()))
+def test_forward_mode_derivatives_and_traces_are_refused(name):
+    """a dual tensor's requires_grad is False, and its derivative would be lost; a trace would keep the empty output"""
+    from torch.autograd import forward_ad
+    call, tensors = _calls()[name]
+    for k, t in enumerate(tensors):
+        with forward_ad.dual_level():
+            args = list(tensors)
+            args[k] = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*args)
+            with pytest.raises(RuntimeError, match="no CPU path"):   # no derivative in sight
+                call(*tensors)
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(call, tuple(tensors))
+
+
+def test_clipping_in_place_refuses_a_dual_gradient():
+    from torch.autograd import forward_ad
+    p = torch.nn.Parameter(torch.zeros(3))
+    with forward_ad.dual_level():
+        p.grad = forward_ad.make_dual(torch.ones(3), torch.ones(3))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.clip_grad_norm_([p], 1.0)
