@@ -24,12 +24,14 @@ __global__ __launch_bounds__(256, 3) void linear_kernel(Layer l, const float* __
     each<TILE>(acc, m0, l.M, n0, l.N, [&](int m, int n, float v) { y[(i64)m * l.N + n] = v + (b ? b[n] : 0.0f); });
 }
 
-// Few tiles: smaller ones, whose 4 waves share k
+// Few tiles: smaller ones, whose 4 waves share k.  2^29 rows and more (of up to 16 outputs) are more workgroups than one axis of a grid takes
 template <int S, int C, bool WIDE>
-__global__ __launch_bounds__(256, 3) void linear_few_kernel(Layer l, const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b, float* __restrict__ y) {
+__global__ __launch_bounds__(256, 3) void linear_few_kernel(Layer l, uint32_t tiles, const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                            float* __restrict__ y) {
     __shared__ __attribute__((aligned(16))) float lds[step_floats<S, C>()];
+    if (block_at() >= tiles) return;
     const int n_tiles = (l.N + 16 * C - 1) / (16 * C);
-    const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const uint32_t tile = tile_of((uint32_t)block_at(), tiles);
     const int n0 = tile % n_tiles * (16 * C), m0 = tile / n_tiles * (16 * S);
     f32x4 acc[C][S] = {};
     step_product<S, C, WIDE>(
@@ -148,9 +150,9 @@ int32_t dsp_linear_forward(void* stream, int64_t rows, int64_t inputs, int64_t o
         const int S = cdiv(l.M, 32) * across >= 256 ? 2 : 1;
 #define DSP_FEW(S, C)                                                                                                                          \
     do {                                                                                                                                       \
-        const dim3 grid((unsigned)(cdiv(l.M, 16 * S) * across));                                                                               \
-        if (wide) hipLaunchKernelGGL((linear_few_kernel<S, C, true>), grid, dim3(256), 0, s, l, x, weight, bias, y);                           \
-        else hipLaunchKernelGGL((linear_few_kernel<S, C, false>), grid, dim3(256), 0, s, l, x, weight, bias, y);                               \
+        const uint32_t tiles = (uint32_t)(cdiv(l.M, 16 * S) * across);                                                                         \
+        if (wide) hipLaunchKernelGGL((linear_few_kernel<S, C, true>), grid_of(tiles), dim3(256), 0, s, l, tiles, x, weight, bias, y);          \
+        else hipLaunchKernelGGL((linear_few_kernel<S, C, false>), grid_of(tiles), dim3(256), 0, s, l, tiles, x, weight, bias, y);              \
     } while (0)
         if (narrow) { if (S == 2) DSP_FEW(2, 1); else DSP_FEW(1, 1); }
         else { if (S == 2) DSP_FEW(2, 4); else DSP_FEW(1, 4); }

@@ -753,6 +753,32 @@ def test_linear_shapes_views_and_missing_parts(ops):
     assert torch.isnan(y[7]).all() and int(torch.isnan(y).sum()) == 32
 
 
+@pytest.mark.parametrize("inputs, outputs", [(2, 2), (4, 1)])
+def test_linear_of_rows_along_two_axes_of_a_grid(ops, inputs, outputs):
+    """2^29 rows and more; whole numbers, whose sums are exact"""
+    rows = 2 ** 29 + 37
+    whole = lambda *shape: torch.randint(-1, 2, shape, device=DEV, dtype=torch.int8).float()
+    x, w, b = whole(rows, inputs), torch.tensor([[2.0, -3.0, 5.0, -7.0], [11.0, 13.0, -17.0, 19.0]], device=DEV)[:outputs, :inputs], torch.tensor([23.0, -29.0], device=DEV)[:outputs]
+    x.requires_grad_()
+    w, b = w.contiguous().requires_grad_(), b.clone().requires_grad_()
+    y = ops.linear(x, w, b)
+    with torch.no_grad():
+        for o in range(outputs):
+            want = torch.full((rows,), float(b[o]), device=DEV)
+            for i in range(inputs):
+                want += x[:, i] * float(w[o, i])
+            assert torch.equal(y[:, o], want)
+        del want
+        g = whole(rows, outputs)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+        del y
+        for i in range(inputs):
+            assert torch.equal(dx[:, i], sum(g[:, o] * float(w[o, i]) for o in range(outputs)))
+            for o in range(outputs):
+                assert float(dw[o, i]) == float((g[:, o] * x[:, i]).sum(dtype=torch.float64))
+        assert torch.equal(db.double(), g.sum(0, dtype=torch.float64))
+
+
 @pytest.mark.parametrize("what", ["embedding", "loss", "lstm"])
 def test_gradients_against_differences(ops, what):
     """f(v + e d) - f(v - e d) over 2 e along a random direction d: the difference quotient is off by e^2 of the third derivative, and by
