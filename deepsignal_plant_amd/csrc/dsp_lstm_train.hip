@@ -24,11 +24,13 @@ namespace {
 struct Shape { int B, T, I, H, dirs; };
 struct Weights { const float *w_ih[2], *w_hh[2], *b_ih[2], *b_hh[2]; };
 
-// gates = W_ih x + b_ih + b_hh, all steps
-template <int TILE, bool FAST> __global__ __launch_bounds__(256, 3) void lstm_inputs_kernel(Shape s, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
+// gates = W_ih x + b_ih + b_hh, all steps.  (2^30 rows of both directions are more workgroups than one axis of a grid takes)
+template <int TILE, bool FAST>
+__global__ __launch_bounds__(256, 3) void lstm_inputs_kernel(Shape s, uint32_t tiles, const float* __restrict__ x, Weights w, float* __restrict__ gates) {
     __shared__ __attribute__((aligned(16))) float lds[2 * half_floats<true, true, TILE>()];
+    if (block_at() >= tiles) return;
     const int M = s.B * s.T, N = 4 * s.H, n_tiles = (N + TILE - 1) / TILE;
-    const uint32_t tile = tile_of(blockIdx.x, gridDim.x);
+    const uint32_t tile = tile_of((uint32_t)block_at(), tiles);
     const int n0 = tile % (n_tiles * s.dirs), d = n0 / n_tiles, at = (n0 - d * n_tiles) * TILE, m0 = tile / (n_tiles * s.dirs) * TILE;
     f32x16 acc[TILE / 64][TILE / 64] = {};
     product<true, true, TILE, FAST>({x, M, s.I}, {w.w_ih[d], N, s.I}, m0, at, 0, s.I, lds, acc, Nothing());
@@ -649,7 +651,8 @@ int32_t dsp_lstm_forward(void* stream, const dsp_lstm_layer* l, const float* x, 
     if (!fused) {
         const int tile = tile_for(M, N * s.dirs);
         const bool fast = input_wide && s.I % kStep == 0;   // a line's last 16 values are all its own
-        DSP_TILES(lstm_inputs_kernel, tile, fast, cdiv(M, tile) * cdiv(N, tile) * s.dirs, q, s, x, w, gates);
+        const i64 tiles = cdiv(M, tile) * cdiv(N, tile) * s.dirs;
+        DSP_TILES_ON(lstm_inputs_kernel, tile, fast, grid_of(tiles), q, s, (uint32_t)tiles, x, w, gates);
     }
     if (!fused && whole_forward(s)) {
         const dim3 grid((unsigned)(cdiv(s.B, 4) * s.dirs)), block(64 * (unsigned)cdiv(s.H, 16));

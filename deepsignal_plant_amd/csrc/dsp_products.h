@@ -285,13 +285,14 @@ inline bool aligned16(const void* p) { return (size_t)p % 16 == 0; }
 
 // tiles of 128 x 128 where they fill the device twice, else of 64 x 64
 inline int tile_for(i64 m, i64 n) { return cdiv(m, 128) * cdiv(n, 128) >= 512 ? 128 : 64; }
-#define DSP_TILES(kernel, tile, fast, blocks, s, ...)                                                                                   \
+#define DSP_TILES_ON(kernel, tile, fast, grid, s, ...)                                                                                  \
     do {                                                                                                                                \
-        if (tile == 128 && fast) hipLaunchKernelGGL((kernel<128, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);       \
-        else if (tile == 128) hipLaunchKernelGGL((kernel<128, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);         \
-        else if (fast) hipLaunchKernelGGL((kernel<64, true>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                  \
-        else hipLaunchKernelGGL((kernel<64, false>), dim3((unsigned)(blocks)), dim3(256), 0, s, __VA_ARGS__);                           \
+        if (tile == 128 && fast) hipLaunchKernelGGL((kernel<128, true>), grid, dim3(256), 0, s, __VA_ARGS__);                           \
+        else if (tile == 128) hipLaunchKernelGGL((kernel<128, false>), grid, dim3(256), 0, s, __VA_ARGS__);                             \
+        else if (fast) hipLaunchKernelGGL((kernel<64, true>), grid, dim3(256), 0, s, __VA_ARGS__);                                      \
+        else hipLaunchKernelGGL((kernel<64, false>), grid, dim3(256), 0, s, __VA_ARGS__);                                               \
     } while (0)
+#define DSP_TILES(kernel, tile, fast, blocks, s, ...) DSP_TILES_ON(kernel, tile, fast, dim3((unsigned)(blocks)), s, __VA_ARGS__)
 
 // A sum over K rows in parts: about 768 workgroups (3 a CU) of the tiles of M by (n0 | n1), and no more than 4,096 products in a row
 struct Split { int tile, parts, per_part; };

@@ -699,6 +699,20 @@ def test_lstm_empty_batch_and_views(ops):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_lstm_of_rows_along_two_axes_of_a_grid(ops):
+    """2^30 - 64 rows of inputs in both directions.  One unit: a gate's argument is four products and sums, off by 8 U of their size
+    (below 2 here), the gates' functions by 4 U each, and a step hands what it is off by on, by no more than itself: 32 U a step"""
+    B, T = 3933120, 273
+    x = torch.randn(B, 1, 1, device=DEV).expand(B, T, 1) * torch.linspace(-1.0, 1.0, T, device=DEV)[:, None]
+    _, ws, _, _, _ = lstm_case(1, 1, 1, 1, seed=4)
+    with torch.no_grad():
+        y, hn, cn = ops.lstm(x, [w.to(DEV) for w in ws])
+    at = torch.cat([torch.arange(2000), torch.randint(0, B, (2000,), generator=gen(1)), torch.arange(B - 2000, B)])
+    want = plain_lstm(x[at.to(DEV)].double().cpu(), [w.double() for w in ws], None, None)
+    for got, w in zip((y[at.to(DEV)], hn[:, at.to(DEV)], cn[:, at.to(DEV)]), want):
+        close(got, w, 32 * U * T)
+
+
 # ---- linear ------------------------------------------------------------------------------------------------------------------------
 def check_linear(ops, shape, inputs, outputs, bias=True, seed=1):
     """each value is a sum of n products: off by at most n U of the sum of their sizes, and once more by the bias"""
