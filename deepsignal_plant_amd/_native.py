@@ -79,6 +79,16 @@ def lib():
         raise RuntimeError("%s implements C-ABI version %d, this package binds version %d (include/dsp_amd.h "
                            "DSP_AMD_ABI_VERSION): rebuild it with `make -C deepsignal_plant_amd/csrc`"
                            % (LIB_PATH, L.dsp_abi_version(), ABI_VERSION))
+    try:
+        _bind(L)
+    except AttributeError as e:   # entry points are added within a version (what it had stays as it was), so an older library can be of this one
+        raise RuntimeError("%s is older than this package (%s): rebuild it with `make -C deepsignal_plant_amd/csrc`" % (LIB_PATH, e)) from None
+    _lib = L
+    return L
+
+
+def _bind(L):
+    """the types of every entry point"""
     L.dsp_weight_count.restype = ctypes.c_int32
     L.dsp_weight_count.argtypes = [ctypes.POINTER(ModelCfg)]
     L.dsp_weight_spec.restype = ctypes.c_int32
@@ -302,8 +312,6 @@ def lib():
         fn.restype, fn.argtypes = restype, argtypes
     L.dsp_debug_range_probe.restype = ctypes.c_int32
     L.dsp_debug_range_probe.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]
-    _lib = L
-    return L
 
 
 def range_probe(device: int = 0):

@@ -23,7 +23,8 @@ extern "C" {
 #endif
 
 #define DSP_AMD_ABI_VERSION 3   /* 2: dsp_init_state.site_keys; 3: dsp_model_query, dsp_device_pci_bdf / _uuid, dsp_profile_enable
-                                   mode 2 (round 5's additions, numbered in round 6), DSP_EBOUNDS */
+                                   mode 2 (round 5's additions, numbered in round 6), DSP_EBOUNDS.  The operators of a training step were
+                                   added to version 3 without a change to what it had: whoever resolves them by name checks for each */
 
 typedef enum dsp_status {
     DSP_OK = 0,

@@ -24,6 +24,26 @@ def test_library_exports_every_declared_symbol():
     assert lib.dsp_abi_version() == 3
 
 
+def test_an_older_library_of_the_same_version_says_what_it_lacks(tmp_path):
+    """a library that answers with this version and has all entry points but the newest ones: the loader's own error, which names it and
+    what is missing, not a bare AttributeError"""
+    import subprocess
+    import sys
+    from deepsignal_plant_amd import _native
+    lacks = "dsp_clip_grad_norm"
+    src = str(tmp_path / "old.c")
+    with open(src, "w") as f:
+        f.write("int dsp_abi_version(void) { return %d; }\n" % _native.ABI_VERSION)
+        f.write("".join("void %s(void) {}\n" % s for s in declared_symbols() if s not in ("dsp_abi_version", lacks)))
+    so = str(tmp_path / "libold.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", so, src], check=True)
+    r = subprocess.run([sys.executable, "-c", "from deepsignal_plant_amd import _native; _native.lib()"], cwd=ROOT, capture_output=True, text=True,
+                       env=dict(os.environ, DSP_AMD_LIB=so))
+    assert r.returncode != 0
+    last = r.stderr.strip().splitlines()[-1]
+    assert last.startswith("RuntimeError") and so in last and lacks in last and "rebuild" in last, r.stderr[-1000:]
+
+
 def test_weight_spec_and_flops_match_oracle_spec():
     from deepsignal_plant_amd.models import ModelBiLSTM
     from oracle import forward_np as onp
