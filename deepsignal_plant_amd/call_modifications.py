@@ -445,11 +445,20 @@ def _call_mods_file(args, rank, local_rank, world):
 def _make_freq(args, dev, world, nthreads):
     """--freq_file: (host aggregator, device aggregator).  Device (default): the calls stay in HBM as records and are
     reduced there, sharded over the ranks (call_mods_freq.DeviceSiteFrequency).  Host (--freq_on host): the native host
-    table; with several ranks it is fed from the merged per-read file by rank 0."""
+    table; with several ranks it is fed from the merged per-read file by rank 0.
+    Ranks that share a GPU take the host table too (the same bytes): a run of two of them with the device aggregator has gone
+    silent for good, and why is not known -- its collectives and kernels, run on the host, end (tests/test_freq_ranks.py)."""
     if not getattr(args, "freq_file", None):
         return None, None
     from .call_mods_freq import DeviceSiteFrequency, SiteFrequency
     if getattr(args, "freq_on", "device") == "device":
+        if dsp_dist.ranks_share_gpus(world):   # the same answer on every rank, before any collective of the aggregator
+            import torch.distributed as dist
+            if dist.get_rank() == 0:
+                sys.stderr.write("[call_freq] %d ranks share the visible GPUs: --freq_file will be computed from the per-read file by the "
+                                 "host table\n" % world)
+            args._freq_from_file = True
+            return None, None
         return None, DeviceSiteFrequency(args.prob_cf, dev, nthreads)
     return (SiteFrequency(args.prob_cf) if world == 1 else None), None
 
@@ -924,7 +933,8 @@ def add_call_mods_args(p):
     g.add_argument("--freq_on", type=str, default="device", choices=["device", "host"],
                    help="where --freq_file is aggregated: 'device' (default) keeps the calls in HBM as records, deals them to "
                         "the ranks by site (one RCCL all_to_all) and reduces them there; 'host' = the native host table "
-                        "(with several ranks: rank 0 re-reads the merged per-read file).  Same bytes either way")
+                        "(with several ranks: rank 0 re-reads the merged per-read file), which ranks that share a GPU take as well.  Same "
+                        "bytes either way")
     g.add_argument("--prob_cf", type=float, default=0.5, help="call_freq threshold on abs(prob1-prob0), default 0.5")
     g.add_argument("--freq_bed", action="store_true", default=False, help="--freq_file in bedMethyl format")
     g.add_argument("--freq_sort", action="store_true", default=False, help="sort --freq_file by chromosome and position")

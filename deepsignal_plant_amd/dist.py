@@ -60,6 +60,14 @@ def init_process_group(world, rank, dev_index, ndev):
     return dist.get_backend()
 
 
+def ranks_share_gpus(world):
+    """several ranks whose group fell back to gloo: init_process_group does that where fewer GPUs than ranks are visible"""
+    if world <= 1:
+        return False
+    import torch.distributed as dist
+    return dist.is_available() and dist.is_initialized() and dist.get_backend() != "nccl"
+
+
 def visible_gpu_count():
     """GPUs this process would see, WITHOUT loading the HIP runtime (the launchers decide how many ranks to start before
     anything may touch the GPU: a process that initialised the GPU must not start replacing itself).  The device
