@@ -18,10 +18,11 @@ def pytest_configure(config):
 
 # Several ranks that share one GPU and reduce --freq_file on it: the first run of such a test on the GPU since the ranks' names
 # travel as json (before, the gather raised TypeError) wrote nothing for 180 seconds after its two-rank launch and was ended.  Whether
-# a rank or the GPU waits for something is not shown, so none of these runs on a GPU until it is.
+# a rank or the GPU waits for something is not shown, so none of these runs on a GPU until it is.  What they hold of one rank is in
+# test_gpu_one_rank.py; the exchange of the ranks runs on the CPU in test_freq_ranks.py.
 SHARED_GPU_FREQ = {
     "test_gpu_canary.py": ("test_the_pipeline_under_the_slot_canary_writes_the_same_bytes",),
-    "test_gpu_cli.py": ("test_cli_fused_freq_file_equals_call_freq_on_the_result", "test_cli_binary_feature_container_gives_the_same_calls_as_the_tsv",
+    "test_gpu_cli.py": ("test_cli_fused_freq_file_equals_call_freq_on_the_result",
                         "test_two_ranks_on_a_foreign_gz_keep_the_input_order_and_the_call_freq_bytes",
                         "test_device_call_freq_falls_back_to_the_host_table_past_its_hbm_budget", "test_cli_on_empty_one_row_and_fewer_rows_than_ranks"),
     "test_gpu_parse.py": ("test_cli_gives_the_same_bytes_whichever_side_parses",),
