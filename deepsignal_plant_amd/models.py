@@ -118,8 +118,11 @@ class ModelBiLSTM(object):
         if device is not None:
             self.device = device
         if self._leaves is not None:
+            dev = torch.device("cuda", self._device_index())
             for v in self._leaves.values():
-                v.data = v.data.to(torch.device("cuda", self._device_index()))
+                grad, v.grad = v.grad, None
+                v.data = v.data.to(dev)
+                v.grad = None if grad is None else grad.to(dev)
         if not self._training:
             self._ensure_handle()
         return self

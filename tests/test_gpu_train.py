@@ -255,6 +255,29 @@ def test_inference_sees_writes_that_leave_no_mark_on_the_parameters():
         moved("a replayed step")
 
 
+def test_cuda_brings_the_gradients_along():
+    """parameters and gradients that lie elsewhere (here: on the host) come to the model's GPU together, and keep their values"""
+    from deepsignal_plant_amd import train_ops as ops
+    cfg, m, _ = build(hidden_size=48, num_layers1=1)
+    ins, labels = batch(cfg, 20)
+    dev = [t.to(DEV) for t in ins]
+    m.train()
+    ops.cross_entropy(m(*dev)[0], labels.to(DEV)).backward()
+    params = m.parameters()
+    want = [(p.detach().clone(), p.grad.clone()) for p in params]
+    none = params[3]
+    none.grad = None
+    for p in params:
+        grad, p.grad = p.grad, None
+        p.data = p.data.cpu()
+        p.grad = None if grad is None else grad.cpu()
+    m.cuda(0)
+    for p, (v, g) in zip(params, want):
+        assert torch.equal(p.detach(), v) and (p is none) == (p.grad is None) and (p.grad is None or torch.equal(p.grad, g))
+    torch.optim.SGD(params, lr=0.1).step()
+    assert torch.equal(m.eval()(*dev)[0], m(*dev)[0])
+
+
 def test_a_captured_inference_pass_outlives_the_weights_it_was_captured_with():
     """the parameters move on after the capture: eager calls serve them, the replayed pass still has its own weights and workspace, with
     memory taken and given back in between"""
