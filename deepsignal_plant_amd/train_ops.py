@@ -52,14 +52,13 @@ def _refuse_unseen(who, tensors):
 
 
 def _one_gpu(who, *tensors):
-    """the index of the tensors' GPU (None among them: not given)"""
+    """the index of the tensors' GPU"""
     _refuse_unseen(who, tensors)
     dev = -1
     for t in tensors:
-        if t is None:
-            continue
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s: expected a tensor, got %s" % (who, type(t).__name__))
+    for t in tensors:
         at = t.get_device()
         if at != dev or dev < 0:
             if at < 0:
@@ -219,7 +218,7 @@ def lstm(x, weights, h0=None, c0=None):
     weights = list(weights)
     if len(weights) not in (4, 8):
         raise ValueError("lstm: expected the 4 weights of one direction or the 8 of two, got %d" % len(weights))
-    given = [t for t in (x, h0, c0, *weights) if t is not None]
+    given = [x, *weights, *(t for t in (h0, c0) if t is not None)]
     _one_gpu("lstm", *given)
     if set(map(_dtype, given)) != {torch.float32}:
         raise ValueError("lstm: tensors must be float32")
@@ -271,9 +270,10 @@ class _Linear(torch.autograd.Function):
 def linear(x, weight, bias=None):
     """x weight^T + bias: [..., outputs] for x [..., inputs], weight [outputs, inputs], bias [outputs]; float32, at most 16,384 inputs
     and outputs.  (torch's own bias gradient is a sum that clears flags by a memset: captured into a graph, its replays went wrong here.)"""
-    _one_gpu("linear", x, weight, bias)
-    for t in (x, weight, bias):
-        if t is not None and t.dtype != torch.float32:
+    given = (x, weight) if bias is None else (x, weight, bias)
+    _one_gpu("linear", *given)
+    for t in given:
+        if t.dtype != torch.float32:
             raise ValueError("linear: tensors must be float32, got %s" % t.dtype)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError("linear: x must be [..., inputs] and weight [outputs, inputs], got %s and %s" % (list(x.shape), list(weight.shape)))
@@ -333,7 +333,7 @@ def cross_entropy(logits, labels, weight=None, ignore_index=-100, reduction="mea
     gradient of zeros; reduction "mean" divides by the sum of the other labels' weights (NaN where there are none).  A label that
     is no class makes its row's loss and gradient NaN.  Where the logits require a gradient it is computed with the loss, for
     an upstream gradient of 1; another one makes the backward pass compute it again from the logits."""
-    _one_gpu("cross_entropy", logits, labels, weight)
+    _one_gpu("cross_entropy", logits, labels, *(() if weight is None else (weight,)))
     if logits.dim() != 2 or logits.dtype not in _FLOAT or logits.shape[1] < 1:
         raise ValueError("cross_entropy: logits must be [n, classes] in float32, bfloat16 or float16, got %s %s" % (list(logits.shape), logits.dtype))
     if tuple(labels.shape) != (logits.shape[0],) or labels.dtype not in _LABEL:

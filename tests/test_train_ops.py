@@ -223,3 +223,20 @@ def test_clipping_in_place_refuses_a_dual_gradient():
         p.grad = forward_ad.make_dual(torch.ones(3), torch.ones(3))
         with pytest.raises(RuntimeError, match="forward-mode"):
             ops.clip_grad_norm_([p], 1.0)
+
+
+@pytest.mark.parametrize("name", sorted(_calls()))
+def test_what_is_not_there_or_no_tensor_is_refused(name):
+    """None and a list in every required place: ValueError, with the operator's name"""
+    call, tensors = _calls()[name]
+    optional = {"lstm": (5, 6), "linear": (2,), "cross_entropy": (1,)}.get(name, ())
+    for k in range(len(tensors)):
+        for wrong in ([None] if k not in optional else []) + [[1.0, 2.0]]:
+            args = list(tensors)
+            args[k] = wrong
+            # every other tensor is on the host: whichever is met first is refused, and none as if it had an attribute that it lacks
+            with pytest.raises((ValueError, RuntimeError), match=name):
+                call(*args)
+    for wrong in (None, [1.0]):
+        with pytest.raises(ValueError, match=name):
+            call(*[wrong] * len(tensors))
