@@ -143,9 +143,9 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
         raise ValueError("embedding: tokens must be uint8, uint16, int32, int64 or float32, got %s" % tokens.dtype)
     if weight.dtype not in _FLOAT or weight.dim() != 2:
         raise ValueError("embedding: weight must be [rows, dim] in float32, bfloat16 or float16, got %s %s" % (list(weight.shape), weight.dtype))
-    scale = float(scale)
+    scale = ctypes.c_float(float(scale)).value   # as the kernels get it
     if not math.isfinite(scale):
-        raise ValueError("embedding: scale must be finite")
+        raise ValueError("embedding: scale must be finite in float32")
     pad = -1   # none
     if padding_idx is not None:
         pad = int(padding_idx)

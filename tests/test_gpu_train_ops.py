@@ -193,6 +193,18 @@ def test_embedding_offsets_past_32_bits(ops):
     assert float(dw[-1, -1]) == 2.0 and int((dw != 0).sum()) == 1
 
 
+def test_embedding_scales(ops):
+    """any finite float32, a tensor of one value among them; one that is finite in 64 bits alone would make every row infinite"""
+    t, w = tokens_of(50, 16), table(16, 4)
+    for scale in (0.0, -2.5, 1e-30, 1e30, torch.tensor(0.75)):
+        check_embedding(ops, t, w, scale=float(scale))
+        assert torch.equal(ops.embedding(t, w, scale=scale), ops.embedding(t, w, scale=float(scale)))
+    assert torch.isfinite(ops.embedding(t, w * 0.01, scale=3.4028234e38)).all()
+    for scale in (1e39, -1e300, math.inf, math.nan):
+        with pytest.raises(ValueError, match="finite in float32"):
+            ops.embedding(t, w, scale=scale)
+
+
 def test_embedding_of_tokens_along_two_axes_of_a_grid(ops):
     """more workgroups than one axis takes, forward and where the runs are joined; sums of small whole numbers are exact"""
     n = 2 ** 25 + 7
