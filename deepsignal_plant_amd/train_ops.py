@@ -408,6 +408,13 @@ class _Pieces(object):
                 raise ValueError("%s: an output overlaps a gradient (clip_grad_norm_ works in place)" % who)
 
 
+class _Reaches(object):
+    """the memory from a strided tensor's first value to its last"""
+
+    def __init__(self, tensors):
+        self.spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in tensors if t.numel())
+
+
 def _run_clip(dev, like, grads, outs, max_norm):
     n, L, numels = len(grads.ptrs), nat.lib(), grads.numels.buffer_info()[0]
     norm = like.new_empty((), dtype=torch.float32)
@@ -441,7 +448,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     """(norm, clipped): min(1, max_norm / (norm + 1e-6)) times every gradient, written into other tensors.
 
     out: one contiguous tensor for each gradient, of its shape, in its type or in float32 (the gradients an optimizer with
-    32-bit weights takes); new ones where it is not given.  The gradients are left as they are."""
+    32-bit weights takes); new ones where it is not given.  The gradients are left as they are: no output may lie in the memory
+    that one of them spans."""
     who, grads = "clip_grad_norm", list(grads)
     max_norm = _max_norm(who, max_norm)
     if not grads:
@@ -464,12 +472,15 @@ def clip_grad_norm(grads, max_norm, out=None):
     for g, o in set(zip(map(_dtype, grads), map(_dtype, out))):
         if o is not g and o is not torch.float32:
             raise ValueError("clip_grad_norm: an output must be of its gradient's type or float32")
-    if not all(map(torch.Tensor.is_contiguous, grads)):
+    strided = [g for g in grads if not g.is_contiguous()]
+    if strided:
         grads = [g.contiguous() for g in grads]
     ins = _Pieces(grads)
     outs = _Pieces(out, ins)
     outs.check_apart(who)
     outs.check_apart_from(who, ins)
+    if strided:
+        outs.check_apart_from(who, _Reaches(strided))
     norm = _run_clip(dev, grads[0], ins, outs, max_norm)
     increment_version(out)   # as torch's own writes do: a graph that saved one of them notices
     return norm, out

@@ -507,6 +507,21 @@ def test_clip_orders_and_strides(ops):
     close(g, (w := torch.randn(40, 30, generator=gen(1)).double()) / (w.norm() + 1e-6), 2.0 ** -22)
 
 
+def test_clip_outputs_over_strided_gradients(ops):
+    """a transposed gradient and one with gaps are copied for the kernels; an output over the gradient itself is refused all the same,
+    and none of its values has changed"""
+    buf = torch.randn(40, 30, generator=gen(1)).to(DEV)
+    keep = buf.clone()
+    for g, o in ((buf.t(), buf.view(30, 40)), (buf[:, ::2], buf.view(-1)[:600].view(40, 15)), (buf[1:, :10], buf.view(-1)[700:1090].view(39, 10))):
+        with pytest.raises(ValueError, match="overlaps a gradient"):
+            ops.clip_grad_norm([g], 1.0, out=[o])
+        assert torch.equal(buf, keep)
+    norm, (o,) = ops.clip_grad_norm([buf[:20, ::2]], 1.0, out=[buf.view(-1)[600:900].view(20, 15)])   # behind it
+    want = keep[:20, ::2].double().cpu()
+    close(o, want / (want.norm() + 1e-6), 2.0 ** -22)
+    assert torch.equal(buf[:20], keep[:20])
+
+
 def test_clip_values_at_the_edges(ops):
     big = [torch.full((100,), 3e38, device=DEV), torch.full((7,), -1e30, device=DEV)]
     norm, out = ops.clip_grad_norm(big, 1.0)
