@@ -304,6 +304,7 @@ def _bind(L):
             ("dsp_linear_workspace", I64, [I64, I64, I64]),
             ("dsp_linear_backward", I32, [P, I64, I64, I64] + [P] * 7 + [I64]),
             ("dsp_cross_entropy_workspace", I64, [I64]),
+            ("dsp_stream_capture_id", ctypes.c_uint64, [P]),
             ("dsp_cross_entropy_forward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, P, P, I64]),
             ("dsp_cross_entropy_backward", I32, [P, I64, I64, P, I32, I64, P, I32, P, I64, I32, P, P, P, I32, P]),
             ("dsp_clip_workspace", I64, [I32, P]),

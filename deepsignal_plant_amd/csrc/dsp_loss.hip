@@ -472,6 +472,16 @@ const char* bad_loss(i64 n, i64 c, i64 stride, int dtype, int label_dtype, int r
 
 extern "C" {
 
+uint64_t dsp_stream_capture_id(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 int64_t dsp_cross_entropy_workspace(int64_t n) { return n < 0 ? refuse("dsp_cross_entropy_workspace", "negative number of rows") : (int64_t)((n + kJoinParts) * sizeof(double2) + kWeightParts * sizeof(double)); }
 
 int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride, const void* labels,

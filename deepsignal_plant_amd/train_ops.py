@@ -84,6 +84,13 @@ def _call(dev, fn, *args):
         nat.check(rc)
 
 
+def _capture(dev):
+    """the number of the capture that the current stream of GPU `dev` is part of; 0: none"""
+    if torch.cuda.current_device() == dev and not torch.cuda.is_current_stream_capturing():
+        return 0
+    return nat.lib().dsp_stream_capture_id(_raw_stream(dev))
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -307,6 +314,7 @@ class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, weight, ignore_index, reduction):
         loss, keep, ctx.unit_grad = _loss_forward(logits, labels, weight, ignore_index, reduction, True)
+        ctx.capture = _capture(logits.get_device())
         ctx.save_for_backward(logits, labels, weight, keep)
         ctx.how = ignore_index, reduction
         return loss
@@ -314,9 +322,10 @@ class _CrossEntropy(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, upstream):
         logits, labels, weight, keep = ctx.saved_tensors
-        # the gradient that the forward pass left is handed out once; a second pass over a retained graph computes its own
+        # the gradient that the forward pass left is handed out once; a second pass over a retained graph computes its own, and so does
+        # one that is captured apart from the forward pass: each of its replays would find what the one before it wrote
         grad, ctx.unit_grad = ctx.unit_grad, None
-        unit = grad is not None
+        unit = grad is not None and ctx.capture == _capture(logits.get_device())
         if not unit:
             grad = logits.new_empty(logits.shape)
         upstream, at = upstream.contiguous(), keep.data_ptr()

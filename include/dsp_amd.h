@@ -633,6 +633,9 @@ int32_t dsp_cross_entropy_forward(void* stream, int64_t n, int64_t c, const void
 int32_t dsp_cross_entropy_backward(void* stream, int64_t n, int64_t c, const void* logits, int32_t dtype, int64_t row_stride,
                                    const void* labels, int32_t label_dtype, const float* weight, int64_t ignore_index, int32_t reduction,
                                    const float* stat, const double* weight_sum, const float* upstream, int32_t skip_unit, void* grad);
+/* The number of the capture that `stream` is part of, 0 where it is none (also after an error).  skip_unit holds where the forward
+ * pass runs before every run of the backward pass: both eager, or both of one captured graph. */
+uint64_t dsp_stream_capture_id(void* stream);
 
 /* norm [1] = the 2-norm over all values of n_tensors arrays; outs (NULL: the norm alone) = min(1, max_norm / (norm + 1e-6)) times
  * them.  grads, outs, numels, dtypes, out_dtypes are HOST tables; an output has its gradient's type or float32, and may be its

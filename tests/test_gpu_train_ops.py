@@ -440,6 +440,38 @@ def test_loss_of_rows_along_two_axes_of_a_grid(ops, n, c, more):
         assert torch.equal(l, loss[part]) and torch.equal(torch.autograd.grad(l, e, torch.ones_like(l))[0], dx[part])
 
 
+@pytest.mark.parametrize("n, c, dtype", [(40, 2, F32), (300, 300, BF16), (7, 40001, F32)])
+@pytest.mark.parametrize("forward", ["eager", "captured apart"])
+def test_loss_backward_captured_by_itself(ops, n, c, dtype, forward):
+    """replayed under one upstream gradient after another: each replay is the gradient for its own, whatever the one before it was"""
+    x, y = logits_of(n, c, dtype), labels_of(n, c)
+    ups = [1.0, 2.0, 1.0, 0.25, 1.0]
+    want = []
+    for u in ups:
+        leaf = x.clone().requires_grad_()
+        want.append(torch.autograd.grad(ops.cross_entropy(leaf, y), leaf, torch.tensor(u, device=DEV))[0])
+    leaf, up = x.clone().requires_grad_(), torch.ones((), device=DEV)
+    side, first, second = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.cross_entropy(leaf, y), leaf, up)
+        if forward == "eager":
+            loss = ops.cross_entropy(leaf, y)
+    torch.cuda.synchronize()
+    if forward != "eager":
+        with torch.cuda.graph(first, stream=side):
+            loss = ops.cross_entropy(leaf, y)
+    with torch.cuda.graph(second, stream=side):
+        dx, = torch.autograd.grad(loss, leaf, up)
+    if forward != "eager":
+        first.replay()
+    for u, w in zip(ups, want):
+        up.fill_(u)
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, w), u
+
+
 # ---- the norm of gradients ---------------------------------------------------------------------------------------------------------
 def check_clip(ops, grads, max_norm, out_dtype=None):
     """the norm is rounded once; an output is the gradient times a factor in 64 bits, rounded to 32 bits and to its type"""
