@@ -699,6 +699,27 @@ def test_lstm_many_sequences(ops, B, T, I, H, dirs, states):
     check_lstm(ops, B, T, I, H, dirs=dirs, states=states)
 
 
+@pytest.mark.parametrize("B,T,I,H,dirs", [(32, 13, 64, 128, 2), (9, 13, 7, 20, 2), (16, 1, 256, 256, 2), (130, 13, 512, 256, 2), (512, 13, 512, 256, 2), (512, 13, 16, 128, 1),
+                                           (1100, 13, 30, 130, 1), (4096, 13, 64, 128, 2), (4096, 13, 48, 256, 2)])
+def test_lstm_holds_32_bits(ops, B, T, I, H, dirs):
+    """as check_lstm, with the errors' signs mixed, so that an operand rounded to 16 bits (2^-9 of itself and more) or a product in fewer than
+    24 shows in every form.  A sum of n products of mixed sign is off by 0.41 n^1/2 U of itself (the partial sums' sizes grow with the root of
+    their length, each addition is off by U 3^-1/2 of one), the gates' functions by 4 U.  h is a quarter of its gates' arguments in size: four
+    times that.  A step hands on less than two thirds of its error: three times.  Twice all that for what is not average: 24 (0.41 n^1/2 + 4) U.
+    A gradient goes through twice as many products, and through the forward's values twice: four times; dW's sum of B T of them on top."""
+    x, ws, h0, c0, grads = lstm_case(B, T, I, H, dirs, seed=B + H)
+    tol = 24 * (0.41 * math.sqrt(I + H + 2) + 4) * U
+    leaves = [t.to(DEV).requires_grad_() for t in (x, h0, c0, *ws)]
+    wide = [t.to(DEV).double().requires_grad_() for t in (x, h0, c0, *ws)]
+    got, want = ops.lstm(leaves[0], leaves[3:], leaves[1], leaves[2]), plain_lstm(wide[0], wide[3:], wide[1], wide[2])
+    for g, w, name in zip(got, want, ("y", "hn", "cn")):
+        near(g, w.cpu(), tol, name)
+    gs = [g.to(DEV) for g in grads]
+    dgot, dwant = torch.autograd.grad(got, leaves, gs), torch.autograd.grad(want, wide, [g.double() for g in gs])
+    for k, (g, w) in enumerate(zip(dgot, dwant)):
+        near(g, w.cpu(), 4 * tol + (0.41 * math.sqrt(B * T) * U if k > 2 else 0), "gradient %d" % k)
+
+
 def test_lstm_saturated_gates_and_large_inputs(ops):
     """weights six times as large; inputs of 1e6 (an un-normalised read), where every gate is 0 or 1"""
     check_lstm(ops, 33, 13, 16, 32, spread=6.0)
