@@ -95,6 +95,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _plain(grad):
+    """a gradient as its values lie in memory: complex arithmetic behind an operator hands back views that stand for their negative"""
+    grad = grad.contiguous()
+    return grad.resolve_neg() if grad.is_neg() else grad
+
+
 def _workspace(like, size):
     return like.new_empty(nat.check(size), dtype=torch.uint8)
 
@@ -130,7 +136,7 @@ class _Embedding(torch.autograd.Function):
         tokens, = ctx.saved_tensors
         rows, dim, scale, padding_idx = ctx.how
         n, L = tokens.numel(), nat.lib()
-        grad = grad.contiguous()
+        grad = _plain(grad)
         out = grad.new_empty((rows, dim))
         size = L.dsp_embedding_workspace(n, rows, dim)
         ws = _workspace(grad, size) if size else None
@@ -199,7 +205,7 @@ class _Lstm(torch.autograd.Function):
     def backward(ctx, gy, ghn, gcn):
         x, c0, gates, cells, *weights = ctx.saved_tensors
         l, L = _layer(x, weights), nat.lib()
-        gy, ghn, gcn = (None if g is None else g.contiguous() for g in (gy, ghn, gcn))
+        gy, ghn, gcn = (None if g is None else _plain(g) for g in (gy, ghn, gcn))
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         states = (l.directions, l.batch, l.hidden)
         dh0 = x.new_empty(states) if ctx.needs_input_grad[1] else None
@@ -265,7 +271,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight = ctx.saved_tensors
         (outputs, inputs), L = weight.shape, nat.lib()
-        rows, grad = x.numel() // inputs, grad.contiguous()
+        rows, grad = x.numel() // inputs, _plain(grad)
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw, db = torch.empty_like(weight), weight.new_empty(outputs) if ctx.has_bias else None
         ws = _workspace(x, L.dsp_linear_workspace(rows, inputs, outputs))
@@ -328,7 +334,7 @@ class _CrossEntropy(torch.autograd.Function):
         unit = grad is not None and ctx.capture == _capture(logits.get_device())
         if not unit:
             grad = logits.new_empty(logits.shape)
-        upstream, at = upstream.contiguous(), keep.data_ptr()
+        upstream, at = _plain(upstream), keep.data_ptr()
         _call(logits.get_device(), nat.lib().dsp_cross_entropy_backward, *_loss_args(logits, labels, weight, *ctx.how), at + 8, at, upstream.data_ptr(), int(unit),
               grad.data_ptr())
         return grad, None, None, None, None
@@ -448,7 +454,7 @@ def grad_norm(grads):
     if not grads:
         raise ValueError("grad_norm: no tensors")
     dev = _check_grads("grad_norm", grads)
-    grads = [g if _is_dense(g) else g.contiguous() for g in grads]
+    grads = [g if _is_dense(g) else g.contiguous() for g in grads]   # (a view that stands for its negative has the same norm)
     return _run_clip(dev, grads[0], _Pieces(grads), None, 0.0)
 
 
@@ -481,9 +487,9 @@ def clip_grad_norm(grads, max_norm, out=None):
     for g, o in set(zip(map(_dtype, grads), map(_dtype, out))):
         if o is not g and o is not torch.float32:
             raise ValueError("clip_grad_norm: an output must be of its gradient's type or float32")
-    strided = [g for g in grads if not g.is_contiguous()]
+    strided = [g for g in grads if not g.is_contiguous() or g.is_neg()]
     if strided:
-        grads = [g.contiguous() for g in grads]
+        grads = [_plain(g) for g in grads]
     ins = _Pieces(grads)
     outs = _Pieces(out, ins)
     outs.check_apart(who)

@@ -424,3 +424,34 @@ def test_what_a_graph_saved_may_not_change():
     ops.clip_grad_norm([torch.ones(5, device=DEV)], 1.0, out=[buf])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_gradients_that_stand_for_their_negative():
+    """complex arithmetic behind an operator's output: the gradient that comes back can be a view with its sign still to be turned, also
+    one of a single value, which is contiguous"""
+    from deepsignal_plant_amd import train_ops as ops
+    gen = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=gen).to(DEV)
+    x, y, table, tokens = r(6, 3), torch.tensor([0, 2, 1, 1, 0, 2], device=DEV), r(16, 1), torch.tensor([5], device=DEV)
+    w, lw = r(1, 3), [r(4, 3), r(4, 1), r(4), r(4)]
+    one = lambda t: (torch.complex(torch.full_like(t, 0.3), t).conj() * (1.5 + 0.5j)).real.sum() * 2.0 + (torch.complex(t, t).conj() * 1j).real.sum()
+
+    def grads(f, leaf, c=None):
+        leaf = leaf.clone().requires_grad_()
+        return torch.autograd.grad(f(leaf) if c is None else one(f(leaf)), leaf)[0]
+    for f, leaf in ((lambda t: ops.cross_entropy(t, y), x), (lambda t: ops.embedding(tokens, t), table), (lambda t: ops.linear(x[:1], t), w),
+                    (lambda t: ops.lstm(x[None, :1], [t, *lw[1:]])[0], lw[0])):
+        d = torch.tensor(0.0, device=DEV, requires_grad=True)
+        k, = torch.autograd.grad(one(d), d)      # `one` is linear: its slope
+        assert (grads(f, leaf, 1) - float(k) * grads(lambda t: f(t).sum(), leaf)).abs().max() < 1e-5
+    g = torch.complex(r(1), r(1)).conj().imag
+    assert g.is_neg() and g.is_contiguous()
+    leaf = x.clone().requires_grad_()
+    loss = ops.cross_entropy(leaf, y)
+    a, b = (torch.autograd.grad(loss, leaf, up.view(()), retain_graph=True)[0] for up in (g, g.resolve_neg()))
+    assert torch.equal(a, b)
+    assert torch.equal(ops.clip_grad_norm([g], 1e9)[1][0], g.resolve_neg())
+    p = torch.nn.Parameter(torch.zeros(1, device=DEV))
+    p.grad = torch.complex(r(1), torch.full((1,), 4.0, device=DEV)).conj().imag
+    ops.clip_grad_norm_(p, 1.0)
+    assert abs(float(p.grad) + 1.0) < 1e-6
