@@ -611,10 +611,11 @@ const char* bad_lstm(i64 B, i64 T, i64 I, i64 H, int dirs) {
 // workgroup on a CU (4 blocks: 12.3 against 11.3 us at 512 sequences of 256 units, the same at 4,096)
 int step_blocks(const Shape& s) { return cdiv(s.B, 32) * cdiv(s.H, 16) * s.dirs >= 256 ? 2 : 1; }
 
-// Forward, many sequences of more than 64 units: 4 at a time pass a CU in so many turns that the step's larger tiles are faster (128 units, both
-// directions, 13 steps: 1,024 sequences 128 us whole and 121 by steps, 2,048: 231 and 221, 4,096: 455 and 373, 16,384: 1,697 and 1,239).
-// Backward the whole form stays ahead (2,382 and 2,648 us at 16,384), and up to 64 units it does in both (439 and 615).
-bool whole_forward(const Shape& s) { return s.H <= kWholeUnits && (s.H <= 64 || cdiv(s.B, 4) * s.dirs < 2048); }
+// Forward, many sequences of more than 64 units: 4 at a time pass a CU in so many turns that the step's larger tiles are faster, from 2,048 in
+// both directions on (13 steps of training, whole and by steps: 128 units 1,536 sequences 178 and 176 us, 2,048: 228 and 232, 3,072: 336 and 302,
+// 16,384: 1,797 and 1,220; 96 units 1,536: 146 and 147, 2,048: 197 and 165; 72 units 1,536: 132 and 133, 2,048: 172 and 164).
+// Backward the whole form stays ahead (2,288 and 2,454 us at 16,384 of 128), and up to 64 units it does in both (530 and 564 forward at 16,384 of 64).
+bool whole_forward(const Shape& s) { return s.H <= kWholeUnits && (s.H <= 64 || cdiv(s.B, 4) * s.dirs < 1024); }
 
 // The forms of many sequences, where the tiles are a workgroup for every CU (forward, whose tiles are larger) or two.  13 steps of both directions, all
 // that belongs to a pass: 2,048 sequences of 1,024 units forward 4,676 -> 3,854 us, back 9,395 -> 7,785; of 256 units, forward 256 tiles, 876 -> 837;

@@ -720,6 +720,11 @@ def test_lstm_holds_32_bits(ops, B, T, I, H, dirs):
         near(g, w.cpu(), 4 * tol + (0.41 * math.sqrt(B * T) * U if k > 2 else 0), "gradient %d" % k)
 
 
+@pytest.mark.parametrize("B,T,I,H,dirs", [(2044, 3, 16, 128, 2), (2045, 3, 16, 128, 2), (2100, 2, 7, 100, 2), (4090, 2, 5, 72, 1), (4093, 2, 16, 65, 1), (2046, 2, 4, 64, 2)])
+def test_lstm_at_the_change_from_one_launch_to_steps(ops, B, T, I, H, dirs):
+    check_lstm(ops, B, T, I, H, dirs=dirs)
+
+
 def test_lstm_saturated_gates_and_large_inputs(ops):
     """weights six times as large; inputs of 1e6 (an un-normalised read), where every gate is 0 or 1"""
     check_lstm(ops, 33, 13, 16, 32, spread=6.0)
