@@ -487,9 +487,10 @@ def clip_grad_norm(grads, max_norm, out=None):
     for g, o in set(zip(map(_dtype, grads), map(_dtype, out))):
         if o is not g and o is not torch.float32:
             raise ValueError("clip_grad_norm: an output must be of its gradient's type or float32")
-    strided = [g for g in grads if not g.is_contiguous() or g.is_neg()]
-    if strided:
-        grads = [_plain(g) for g in grads]
+    strided = []
+    if not all(map(torch.Tensor.is_contiguous, grads)) or any(map(torch.Tensor.is_neg, grads)):
+        strided = [g for g in grads if not g.is_contiguous()]
+        grads = list(map(_plain, grads))
     ins = _Pieces(grads)
     outs = _Pieces(out, ins)
     outs.check_apart(who)
