@@ -159,8 +159,9 @@ class ModelBiLSTM(object):
         for v in (self._leaves or {}).values():
             if set_to_none:
                 v.grad = None
-            elif v.grad is not None:
-                v.grad = torch.zeros_like(v.grad)
+            elif v.grad is not None:   # in place: a captured step adds to these tensors
+                v.grad.detach_()
+                v.grad.zero_()
 
     def _leaf_marks(self):
         return [(v.data_ptr(), v._version) for v in self._leaves.values()]

@@ -278,6 +278,35 @@ def test_cuda_brings_the_gradients_along():
     assert torch.equal(m.eval()(*dev)[0], m(*dev)[0])
 
 
+def test_zero_grad_in_place_and_a_captured_step_that_accumulates():
+    """set_to_none=False clears the tensors that are there: a captured backward pass goes on adding to them"""
+    from deepsignal_plant_amd import train_ops as ops
+    cfg, m, _ = build(hidden_size=48, num_layers1=1)
+    ins, labels = batch(cfg, 64)
+    dev, y = [t.to(DEV) for t in ins], labels.to(DEV)
+    params = m.train().parameters()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = torch.autograd.grad(ops.cross_entropy(m(*dev)[0], y), params)
+    torch.cuda.current_stream().wait_stream(side)
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    grads = [p.grad for p in params]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for p, d in zip(params, torch.autograd.grad(ops.cross_entropy(m(*dev)[0], y), params)):
+            p.grad.add_(d)
+    for _ in range(3):
+        m.zero_grad(set_to_none=False)
+        assert all(p.grad is a and not a.any() for p, a in zip(params, grads))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p.grad, w) for p, w in zip(params, want))
+    m.zero_grad()
+    assert all(p.grad is None for p in params)
+
+
 def test_a_captured_inference_pass_outlives_the_weights_it_was_captured_with():
     """the parameters move on after the capture: eager calls serve them, the replayed pass still has its own weights and workspace, with
     memory taken and given back in between"""
