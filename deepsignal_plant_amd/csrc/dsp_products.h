@@ -189,7 +189,8 @@ struct Nothing { template <class V> __device__ __forceinline__ void operator()(c
 // Every wave takes a quarter of k and the whole tile, so that no value is loaded by two waves.  It loads lines of 128 bytes, 8 rows at a
 // time, 32 values of k ahead, and turns them in LDS of its own into what v_mfma_f32_16x16x4 takes (a lane's 4 consecutive k of one
 // row, as above).  Loaded in that form from memory they would cost the L1 an access for each 16 bytes: 16 neighbouring lanes are 16
-// rows (90 us a step of 4,096 sequences instead of 70).  No wave waits for another until the quarters are joined, in order.  WIDE: rows begin at multiples of 16 bytes and k is one of 4.
+// rows (90 us a step of 4,096 sequences instead of 70).  No wave waits for another until the quarters are joined, in order.
+// WIDE: rows begin at multiples of 16 bytes and k is one of 4.
 constexpr int kLine = 32;   // values of k at a time
 // where 4 values of a row lie in LDS: the 8 places of a row change with the pair of rows, so that 16 rows read at once fall on all banks
 __device__ __forceinline__ int spread(int row, int k) { return row * kLine + (((k >> 2) ^ (row >> 1)) & 7) * 4; }
